@@ -12,11 +12,15 @@ without the library.)
 from .inputs import WORKLOADS, Workload, make_problem  # noqa: F401
 
 _API = ("Attention", "JointAttention", "build_rope_4axis_tables", "rmsnorm_bf16", "rope_4axis_inplace_bf16")
-__all__ = [*_API, "WORKLOADS", "Workload", "make_problem"]
+_PAGED = ("PagedBatch", "PagedKV")
+__all__ = [*_API, *_PAGED, "WORKLOADS", "Workload", "make_problem"]
 
 
 def __getattr__(name):
     if name in _API:
         from . import api          # loads the library (and builds it first when it is stale)
         return getattr(api, name)
+    if name in _PAGED:
+        from . import paged
+        return getattr(paged, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -30,6 +30,27 @@ class AttnStrides(C.Structure):
     _fields_ = [(n, C.c_longlong) for n in ("q_txt", "k_txt", "v_txt", "o_txt", "q_img", "k_img", "v_img", "o_img")]
 
 
+class KvConfig(C.Structure):
+    """struct f2k_kv_config"""
+    _fields_ = [(n, C.c_int) for n in ("n_heads", "n_kv_heads", "head_dim", "page_size", "n_pages", "type", "cache_type",
+                                       "rot_dim", "interleaved", "window")] \
+        + [("scale", C.c_float), ("k_pages", C.c_void_p), ("v_pages", C.c_void_p)] \
+        + [(n, C.c_longlong) for n in ("k_page_stride", "k_head_stride", "k_token_stride",
+                                       "v_page_stride", "v_head_stride", "v_token_stride")] \
+        + [("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class KvBatch(C.Structure):
+    """struct f2k_kv_batch"""
+    _fields_ = [("n_seqs", C.c_int), ("n_tokens", C.c_int), ("max_new", C.c_int), ("table_width", C.c_int),
+                ("table_stride", C.c_longlong), ("cu_seqlens", C.c_void_p), ("kv_lens", C.c_void_p), ("page_table", C.c_void_p)]
+
+
+class KvStrides(C.Structure):
+    """struct f2k_kv_strides: token strides in elements, 0 = dense"""
+    _fields_ = [(n, C.c_longlong) for n in ("q", "k", "v", "q_out", "o")]
+
+
 def _declare(lib: C.CDLL) -> None:
     vp, i, f, sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
     lib.f2k_attn_create.restype = i
@@ -118,6 +139,22 @@ def _declare(lib: C.CDLL) -> None:
     lib.f2k_ipc_close.argtypes = [vp]
     lib.f2k_qk_norm_rope_bf16.restype = i
     lib.f2k_qk_norm_rope_bf16.argtypes = [vp, vp, vp, vp, vp, i, i, i, f, vp]
+    lib.f2k_kv_create.restype = i
+    lib.f2k_kv_create.argtypes = [C.POINTER(KvConfig), C.POINTER(vp)]
+    lib.f2k_kv_destroy.restype = None
+    lib.f2k_kv_destroy.argtypes = [vp]
+    lib.f2k_kv_last_error.restype = C.c_char_p
+    lib.f2k_kv_last_error.argtypes = [vp]
+    lib.f2k_kv_append.restype = i
+    lib.f2k_kv_append.argtypes = [vp] * 9 + [i, f, vp, vp, vp]
+    lib.f2k_kv_workspace_bytes.restype = sz
+    lib.f2k_kv_workspace_bytes.argtypes = [vp, vp]
+    lib.f2k_kv_attend.restype = i
+    lib.f2k_kv_attend.argtypes = [vp] * 7 + [sz, vp]
+    lib.f2k_kv_device_status.restype = i
+    lib.f2k_kv_device_status.argtypes = [vp, C.POINTER(i)]
+    lib.f2k_kv_set_wait_limits.restype = i
+    lib.f2k_kv_set_wait_limits.argtypes = [vp, C.c_longlong]
     lib.f2k_attn_version.restype = C.c_char_p
     lib.f2k_attn_version.argtypes = []
 

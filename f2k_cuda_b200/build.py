@@ -9,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -17,7 +18,8 @@ CSRC = PKG_DIR / "csrc"
 BUILD_DIR = PKG_DIR / "_build"
 LIB_PATH = BUILD_DIR / "libf2k_attn.so"
 
-SOURCES = ["attn_fwd_sm100.cu", "qk_prologue.cu", "capi.cu", "no_alloc.cu", "seqpar.cu", "headswap.cu", "f2k_compat.cpp"]
+SOURCES = ["attn_fwd_sm100.cu", "qk_prologue.cu", "capi.cu", "no_alloc.cu", "seqpar.cu", "headswap.cu",
+           "kv/paged_kv.cu", "kv/kv_append.cu", "kv/paged_token.cu", "f2k_compat.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -62,16 +64,18 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 def _build_locked(verbose: bool) -> Path:
     nvcc = _nvcc()
-    objs = []
+    objs, cmds = [], []
     for src in SOURCES:
-        obj = BUILD_DIR / (src.rsplit(".", 1)[0] + ".o")
+        obj = BUILD_DIR / (src.rsplit(".", 1)[0].replace("/", "_") + ".o")
         cmd = [nvcc, *NVCC_FLAGS, "-x", "cu", "-I", str(REPO_DIR / "include"), "-I", str(CSRC),
                "-I", str(CSRC / "compat"), "-DF2K_ATTN_BUILD", "-c", str(CSRC / src), "-o", str(obj)]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
             print(" ".join(cmd), file=sys.stderr)
-        subprocess.run(cmd, check=True)
+        cmds.append(cmd)
         objs.append(str(obj))
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        list(pool.map(lambda cmd: subprocess.run(cmd, check=True), cmds))
     tmp = LIB_PATH.with_suffix(".so.tmp")       # linked beside the target, then moved into place in one step
     cmd = [nvcc, "-shared", "-o", str(tmp), *objs, "-gencode", "arch=compute_100a,code=sm_100a"]
     subprocess.run(cmd, check=True)

@@ -1,0 +1,19 @@
+// Host-callable launchers of the paged cache's kernels.
+#pragma once
+
+#include "paged_params.h"
+
+#include <cuda_runtime.h>
+
+namespace f2k {
+
+cudaError_t kv_append_launch(const AppendParams& p, PagedType type, PagedType cache, int head_dim, cudaStream_t stream);
+
+// Query rows of a work that the token kernel's variants hold: 16, 32 or 64.
+int         token_rows(long long rows);
+cudaError_t paged_token_prepare(PagedType type, PagedType cache, int head_dim);   // load the kernels on the current device
+// rows: of a tile, one of token_rows(); used_rows: the most that any tile of the call has.
+cudaError_t paged_token_launch(const AttendParams& p, PagedType type, PagedType cache, int head_dim, int rows, int used_rows,
+                               cudaStream_t stream);
+
+}  // namespace f2k

@@ -375,6 +375,98 @@ int f2k_qk_norm_rope_bf16(const void* x, void* y, const void* gamma, const float
                           const float* sin_table, int batch, int seq, int n_heads, float eps,
                           void* stream);
 
+/* ---- paged key/value cache: decoder attention for prompts and for single tokens ---------------
+ * The language model in front of the image model attends causally, with n_heads / n_kv_heads query
+ * heads per key head, over a cache that grows by a prompt and then token by token. The cache is
+ * cut into pages of page_size tokens; a table names the pages of every sequence. A handle stands
+ * for one layer's cache: its shapes, its two page arrays (the caller's memory), the layer's
+ * rotation and window. No counterpart in the reference, whose text encoder recomputes every
+ * prompt with a row-per-block kernel (src/backend/cuda/qwen_attention.cu:49-109).
+ *
+ * f2k_kv_append writes the new tokens of a batch into the cache, f2k_kv_attend attends them; a
+ * layer calls one after the other on one stream. Both read lengths and page table from device
+ * memory only, so that captured calls can be replayed with others. */
+typedef struct f2k_kv f2k_kv; /* opaque */
+
+enum { F2K_BF16 = 0, F2K_F16 = 1, F2K_E4M3 = 2 };
+
+typedef struct f2k_kv_config {
+    int n_heads;       /* query heads, a multiple of n_kv_heads, at most 128 times as many */
+    int n_kv_heads;
+    int head_dim;      /* 64 or 128 */
+    int page_size;     /* tokens: 16, 32, 64, 128 or 256 */
+    int n_pages;
+    int type;          /* of Q, K, V, O and the gains: F2K_BF16 or F2K_F16 */
+    int cache_type;    /* the same, or F2K_E4M3 */
+    int rot_dim;       /* leading elements of a head that the rotation turns: 0 (none) or a multiple of 16 */
+    int interleaved;   /* pairs are neighbours (2i, 2i+1); else (i, i + rot_dim / 2) */
+    int window;        /* a token sees itself and the window - 1 tokens before it; 0: all before it */
+    float scale;       /* of the scores; <= 0 selects 1/sqrt(head_dim) */
+    void* k_pages;     /* [n_pages][n_kv_heads][page_size][head_dim], or any order by the strides below */
+    void* v_pages;
+    /* strides in elements, multiples of 16 bytes; all three 0: dense in the order above */
+    long long k_page_stride, k_head_stride, k_token_stride;
+    long long v_page_stride, v_head_stride, v_token_stride;
+    /* e4m3 only: [n_kv_heads] fp32 on the device, positive; an element stands for its value times its
+     * head's scale. NULL: 1. */
+    const float* k_scale;
+    const float* v_scale;
+} f2k_kv_config;
+
+/* The sequences of a call. Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of
+ * the call's tensors (any number, none included); kv_lens[b] is its length WITH them, so the last of
+ * them is at position kv_lens[b] - 1. Rows behind the last sequence are left as they are. Key j lies
+ * in page page_table[b * table_stride + j / page_size]. Sequences may share pages that nobody appends
+ * to; a page that receives tokens belongs to one sequence.
+ * Lengths that do not fit (negative, longer than the table's row, shorter than the new tokens, rows
+ * outside the call's) and page numbers outside the cache never make a kernel reach outside: such
+ * tokens are not appended, such keys not attended, and f2k_kv_device_status reports it. */
+typedef struct f2k_kv_batch {
+    int n_seqs;
+    int n_tokens;               /* rows of the call's tensors */
+    int max_new;                /* the most new tokens that a sequence has: decides which kernel attends */
+    int table_width;            /* pages in a row of the table */
+    long long table_stride;     /* int32 between rows; 0: table_width */
+    const int32_t* cu_seqlens;  /* [n_seqs + 1]; NULL: one new token per sequence, row b for sequence b */
+    const int32_t* kv_lens;     /* [n_seqs] */
+    const int32_t* page_table;
+} f2k_kv_batch;
+
+/* Token strides in elements (multiples of 8, heads dense); 0 = dense. k and v: n_kv_heads heads. */
+typedef struct f2k_kv_strides {
+    long long q, k, v, q_out, o;
+} f2k_kv_strides;
+
+/* *out is set whenever memory for a handle could be had, so that the message can be read. */
+int         f2k_kv_create(const f2k_kv_config* cfg, f2k_kv** out);
+void        f2k_kv_destroy(f2k_kv* h);
+const char* f2k_kv_last_error(const f2k_kv* h);
+
+/* q_out = rotated (normalised) q; k likewise and v go to the cache. q, q_out: [n_tokens][n_heads][head_dim],
+ * k, v: [n_tokens][n_kv_heads][head_dim]; q_out may be q. gamma_q, gamma_k: [head_dim] gains of a per-head
+ * RMSNorm in front of the rotation, or both NULL for none. cos, sin: fp32 [n_positions][rot_dim / 2], row =
+ * position; NULL with rot_dim 0. fp32 arithmetic, one rounding. */
+int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const void* q, const void* k, const void* v,
+                  const void* gamma_q, const void* gamma_k, const float* cos_table, const float* sin_table,
+                  int n_positions, float eps, void* q_out, const f2k_kv_strides* strides, void* stream);
+
+/* Bytes of workspace that f2k_kv_attend needs for a batch of these n_seqs, n_tokens and max_new. Calls
+ * whose GPU work may overlap need one each. */
+size_t f2k_kv_workspace_bytes(const f2k_kv* h, const f2k_kv_batch* batch);
+
+/* o = softmax(scale q K^T) V over the keys that each token sees; zero for a token that sees none.
+ * lse: fp32 [n_tokens][n_heads], the logarithm of the sum of exp(scale q K^T) (-inf for none), or
+ * NULL. Tokens of a call do not see values of later tokens, but a value that is not finite can make
+ * the outputs of up to 127 tokens before it NaN; what lies in pages beyond kv_lens does not matter. */
+int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const void* q, void* o, float* lse,
+                  const f2k_kv_strides* strides, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Reads and clears the status word of this handle's kernels (0 = clean); synchronises the handle's
+ * device. F2K_ERR_DEVICE and a message when it is not zero. */
+int f2k_kv_device_status(f2k_kv* h, int* status_out);
+/* As f2k_attn_set_wait_limits; these kernels wait for nothing outside their thread block. */
+int f2k_kv_set_wait_limits(f2k_kv* h, long long in_cta_clk);
+
 /* Library identification string (static storage). */
 const char* f2k_attn_version(void);
 
