@@ -19,7 +19,7 @@ BUILD_DIR = PKG_DIR / "_build"
 LIB_PATH = BUILD_DIR / "libf2k_attn.so"
 
 SOURCES = ["attn_fwd_sm100.cu", "qk_prologue.cu", "capi.cu", "no_alloc.cu", "seqpar.cu", "headswap.cu",
-           "kv/paged_kv.cu", "kv/kv_append.cu", "kv/paged_token.cu", "f2k_compat.cpp"]
+           "kv/paged_kv.cu", "kv/kv_append.cu", "kv/paged_token.cu", "kv/paged_prompt_sm100.cu", "f2k_compat.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -21,7 +21,7 @@ struct f2k_kv {
     int           device = -1, sms = 0, page_shift = 0;
     int*          d_status = nullptr;
     long long     wait_clk = 0;
-    CUtensorMap   token_k, token_v;
+    CUtensorMap   token_k, token_v, prompt_k, prompt_v;
 };
 
 namespace {
@@ -39,8 +39,9 @@ int fail_cuda(f2k_kv* h, const char* what, cudaError_t e) { return fail(h, F2K_E
 bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
 // A cache array as [pages][kv heads][128-byte pieces of a row][tokens of a page][piece]: the rows of a box stand one
-// behind the other, 128 (or 64) bytes each, which is how the kernels read a piece of head_dim.
-int encode_pages(f2k_kv* h, CUtensorMap* map, void* base, long long page, long long head, long long tok, int rows) {
+// behind the other, 128 (or 64) bytes each, which is how the kernels read a piece of head_dim. A box has `rows` tokens and
+// `pieces` pieces (0: all).
+int encode_pages(f2k_kv* h, CUtensorMap* map, void* base, long long page, long long head, long long tok, int rows, int pieces) {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
     const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
@@ -49,7 +50,7 @@ int encode_pages(f2k_kv* h, CUtensorMap* map, void* base, long long page, long l
     const cuuint64_t es = c.cache_type == F2K_E4M3 ? 1 : 2, row = c.head_dim * es, piece = row < 128 ? row : 128;
     const cuuint64_t dims[5] = {piece / es, (cuuint64_t)c.page_size, row / piece, (cuuint64_t)c.n_kv_heads, (cuuint64_t)c.n_pages};
     const cuuint64_t strides[4] = {tok * es, piece, head * es, page * es};
-    const cuuint32_t box[5] = {(cuuint32_t)(piece / es), (cuuint32_t)rows, (cuuint32_t)(row / piece), 1, 1}, step[5] = {1, 1, 1, 1, 1};
+    const cuuint32_t box[5] = {(cuuint32_t)(piece / es), (cuuint32_t)rows, (cuuint32_t)(pieces ? pieces : row / piece), 1, 1}, step[5] = {1, 1, 1, 1, 1};
     const CUresult r = reinterpret_cast<EncodeTiledFn>(fn)(
         map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, base, dims, strides, box, step,
         CU_TENSOR_MAP_INTERLEAVE_NONE, piece == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
@@ -104,6 +105,10 @@ Workspace workspace_of(const f2k_kv* h, int rows) {
     return w;
 }
 int group_of(const f2k_kv* h) { return h->cfg.n_heads / h->cfg.n_kv_heads; }
+// Which kernel attends. An e4m3 cache has the token kernel only: its products are fp16 ones on registers.
+bool takes_prompt_kernel(const f2k_kv* h, const f2k_kv_batch* b) {
+    return h->cfg.cache_type != F2K_E4M3 && b->max_new > 1 && (long long)b->max_new * group_of(h) > 64;
+}
 int rows_of(const f2k_kv* h, const f2k_kv_batch* b) { return token_rows((long long)b->max_new * group_of(h)); }
 
 }  // namespace
@@ -159,11 +164,17 @@ int f2k_kv_create(const f2k_kv_config* cfg, f2k_kv** out) {
     if (e != cudaSuccess) return fail_cuda(h, "cudaDeviceGetAttribute", e);
     if (major != 10) return fail(h, F2K_ERR_UNSUPPORTED, "this library contains sm_100a code only (needs a B200-class GPU)");
     e = paged_token_prepare((PagedType)c.type, (PagedType)c.cache_type, c.head_dim);
+    if (e == cudaSuccess && c.cache_type != F2K_E4M3) e = paged_prompt_prepare((PagedType)c.type, c.head_dim);
     if (e != cudaSuccess) return fail_cuda(h, "kernel load", e);
     const int unit = token_unit_keys(c.head_dim * (c.cache_type == F2K_E4M3 ? 1 : 2));
     const int rows = unit < c.page_size ? unit : c.page_size;
-    int rc = encode_pages(h, &h->token_k, c.k_pages, c.k_page_stride, c.k_head_stride, c.k_token_stride, rows);
-    if (rc == F2K_OK) rc = encode_pages(h, &h->token_v, c.v_pages, c.v_page_stride, c.v_head_stride, c.v_token_stride, rows);
+    int rc = encode_pages(h, &h->token_k, c.k_pages, c.k_page_stride, c.k_head_stride, c.k_token_stride, rows, 0);
+    if (rc == F2K_OK) rc = encode_pages(h, &h->token_v, c.v_pages, c.v_page_stride, c.v_head_stride, c.v_token_stride, rows, 0);
+    if (rc == F2K_OK && c.cache_type != F2K_E4M3) {
+        const int most = c.page_size < kPromptTile ? c.page_size : kPromptTile;
+        rc = encode_pages(h, &h->prompt_k, c.k_pages, c.k_page_stride, c.k_head_stride, c.k_token_stride, most, 1);
+        if (rc == F2K_OK) rc = encode_pages(h, &h->prompt_v, c.v_pages, c.v_page_stride, c.v_head_stride, c.v_token_stride, most, 1);
+    }
     if (rc != F2K_OK) return rc;
     e = cudaMalloc(reinterpret_cast<void**>(&h->d_status), kStatusBytes);
     if (e != cudaSuccess) return fail_cuda(h, "cudaMalloc(status)", e);
@@ -210,7 +221,7 @@ int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const void* q, const voi
 }
 
 size_t f2k_kv_workspace_bytes(const f2k_kv* h, const f2k_kv_batch* batch) {
-    if (!h || !h->valid || !batch || batch->max_new <= 0) return 0;
+    if (!h || !h->valid || !batch || batch->max_new <= 0 || takes_prompt_kernel(h, batch)) return 0;
     return workspace_of(h, rows_of(h, batch)).bytes;
 }
 
@@ -231,6 +242,12 @@ int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const void* q, void* o, 
     p.window = c.window, p.scale_log2 = h->scale * 1.4426950408889634f, p.status = h->d_status;
     p.wait_limit_clk = h->wait_clk > 0 ? h->wait_clk : kDefaultWaitClk;
 
+    if (takes_prompt_kernel(h, batch)) {
+        p.tm_k = h->prompt_k;
+        p.tm_v = h->prompt_v;
+        const cudaError_t e = paged_prompt_launch(p, (PagedType)c.type, c.head_dim, batch->max_new, h->sms, static_cast<cudaStream_t>(stream));
+        return e == cudaSuccess ? F2K_OK : fail_cuda(h, "attention launch", e);
+    }
     const int rows = rows_of(h, batch);
     const Workspace ws = workspace_of(h, rows);
     if (!workspace || workspace_bytes < ws.bytes) return fail(h, F2K_ERR_WORKSPACE, "workspace smaller than f2k_kv_workspace_bytes");

@@ -1,0 +1,568 @@
+// Causal attention of prompts over a paged cache, 16-bit types, head_dim 64 or 128, for sm_100a.
+//
+// A tile is 128 query rows of one sequence and key head: 128 / group new tokens with the `group` query heads of the key
+// head side by side (fewer rows where group does not divide 128), so a key and its value are read once for all heads
+// that share them, and the rows of a tile see nearly the same keys. A CTA has two neighbouring tiles, or one, and walks
+// the 128-key tiles between the first key that its first token sees and the last that its last one sees.
+//
+// Roles as in the joint-attention kernel (attn_fwd_sm100.cu): warps 0-3 / 4-7 the softmax of tile 0 / 1 (one thread per
+// row), warp 8 the loader, warp 9 the tcgen05 issuer, one S buffer in tensor memory that the tiles use in turn, P from
+// tensor memory, lazily moved reference maxima. What differs:
+//
+//  * The loader brings a key tile in page by page: a lane per page and 128-byte piece of head_dim looks its page up (a
+//    tile ahead) and issues its own TMA box. Rows of V that no query of the CTA may see - the rest of the last page,
+//    pages in front of a window, pages outside the cache - hold anything, and 0 * NaN is NaN in a product, so the loader
+//    waits for such a tile and clears them before it hands the tile over. That is the last tile, or the first ones of a
+//    window.
+//  * Q is fetched by the softmax groups themselves (the rows of a tile are a gather once group is not a power of two).
+//  * Scores are masked by key number, only in tiles that some row of the warp does not see whole.
+//
+// Long tiles first: the grid's first CTAs are the last tiles of every sequence, which see the most keys.
+#include "../attn_params.h"
+#include "../barrier_look.h"
+#include "../ptx.cuh"
+#include "../softmax_row.cuh"
+#include "kv_launch.h"
+#include "mma_sync.cuh"
+
+#include <cstddef>
+#include <type_traits>
+
+namespace f2k {
+
+using namespace f2k::ptx;
+
+namespace {
+
+constexpr int kThreads = 384, kLoaderWarp = 8, kMmaWarp = 9;
+constexpr int kStages = 4;
+constexpr int kRows = 128, kKeys = kPromptTile;
+constexpr uint32_t kPieceBytes = 128 * 128;             // 128 rows of 128 bytes
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColS = 0, kColP0 = 128, kColP1 = 192, kColO0 = 256, kColO1 = 384;
+constexpr float kLazyThreshold = 8.0f;                  // log2 units
+constexpr int kPParts = 2;
+constexpr int kBoxRing = 8;                             // tiles whose page flags are kept; the loader is at most three ahead
+
+struct Ctl {
+    uint64_t q_full[2];
+    uint64_t kv_full[kStages];
+    uint64_t kv_empty[kStages];
+    uint64_t s_full[2];
+    uint64_t s_free;
+    uint64_t p_full[2][kPParts];
+    uint64_t pv_done[2];
+    uint64_t drain;
+    uint64_t clean;                                     // a V tile that has to be cleared in part has arrived
+    uint32_t tmem_base;
+    uint32_t abort;
+    uint32_t boxes[kBoxRing];                           // pages of a key tile that were fetched, a bit each
+};
+
+struct WarpBarriers {                                   // the MMA warp's side of barrier_look.h
+    volatile uint32_t* abort_flag;
+    long long limit;
+    __device__ __forceinline__ bool test(uint32_t bar_a, uint32_t par_a, uint32_t bar_b, uint32_t par_b) const {
+        return bar_a == bar_b ? mbar_test(bar_a, par_a) : mbar_test2(bar_a, par_a, bar_b, par_b);
+    }
+    __device__ __forceinline__ bool all(bool pred) const { return __all_sync(0xffffffffu, pred) != 0; }
+    __device__ __forceinline__ bool wait(uint32_t bar, uint32_t par) const { return all(mbar_wait(bar, par, abort_flag, limit)); }
+};
+
+// 16 scores -> 8 packed pairs of T and the sum of the unrounded values (softmax_row.cuh has it for bf16).
+template <class T>
+__device__ __forceinline__ void exp_chunk(const uint32_t* s, uint32_t* pk, float c, float neg_mc, float (&sum)[4]) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        float x0, x1, x2, x3;
+        fma2(x0, x1, __uint_as_float(s[i + 0]), __uint_as_float(s[i + 1]), c, c, neg_mc, neg_mc);
+        fma2(x2, x3, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]), c, c, neg_mc, neg_mc);
+        const float p0 = ex2_approx(x0), p1 = ex2_approx(x1), p2 = ex2_approx(x2), p3 = ex2_approx(x3);
+        add2(sum[0], sum[1], sum[0], sum[1], p0, p1);
+        add2(sum[2], sum[3], sum[2], sum[3], p2, p3);
+        pk[i / 2 + 0] = Half16<T>::pack(p0, p1);
+        pk[i / 2 + 1] = Half16<T>::pack(p2, p3);
+    }
+}
+
+// The work of CTA `slot` (of one key head): sequence and first tile. Sequences one behind the other, in each the last
+// tiles first. False: there is none.
+struct Job {
+    SeqView s;
+    int b, tile0;
+    bool two;
+};
+__device__ __forceinline__ bool find_job(const AttendParams& p, int tokens_per_tile, int per_cta, int slot, int lane, Job& job) {
+    const PagedBatch& b = p.batch;
+    int before = 0;
+    for (int b0 = 0; b0 < b.n_seqs; b0 += 32) {
+        const int i = b0 + lane;
+        SeqView s{0, 0, 0, false};
+        if (i < b.n_seqs) s = seq_view(b.cu ? b.cu[i] : i, b.cu ? b.cu[i + 1] : i + 1, b.lens[i], b.n_tokens, (long long)b.table_width << p.page_shift);
+        if (s.bad && lane == i - b0) atomicOr(p.status, (int)kStatusBadLength);
+        const int tiles = (s.n_new + tokens_per_tile - 1) / tokens_per_tile, ctas = (tiles + per_cta - 1) / per_cta;
+        int upto = ctas;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, slot < before + upto);
+        if (here != 0) {
+            const int src = __ffs(here) - 1;
+            const int nth = slot - before - __shfl_sync(0xffffffffu, upto - ctas, src);      // CTA of the sequence
+            const int n = __shfl_sync(0xffffffffu, ctas, src), all = __shfl_sync(0xffffffffu, tiles, src);
+            job.b = b0 + src;
+            job.s.first = __shfl_sync(0xffffffffu, s.first, src);
+            job.s.n_new = __shfl_sync(0xffffffffu, s.n_new, src);
+            job.s.len = __shfl_sync(0xffffffffu, s.len, src);
+            job.tile0 = (n - 1 - nth) * per_cta;
+            job.two = per_cta == 2 && job.tile0 + 1 < all;
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
+    constexpr int kPieces = D / 64;                     // 128-byte pieces of a row
+    constexpr uint32_t kTileBytes = kPieces * kPieceBytes;
+    constexpr uint32_t kSmemQ = 0, kSmemRing = 2 * kTileBytes;
+    constexpr uint32_t kFormat = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Ctl ctl_;
+    Ctl* ctl = &ctl_;
+    const uint32_t raw_addr = smem_u32(smem_raw);
+    const uint32_t smem = (raw_addr + 1023u) & ~1023u;
+    volatile uint32_t* abort_flag = &ctl->abort;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+    const int lane = threadIdx.x & 31;
+    const long long wait_limit = p.wait_limit_clk;
+
+    grid_launch_dependents();
+    if (warp == kLoaderWarp) {
+        constexpr int kBars = offsetof(Ctl, tmem_base) / sizeof(uint64_t);
+        constexpr int kFree = offsetof(Ctl, s_free) / sizeof(uint64_t), kP = offsetof(Ctl, p_full) / sizeof(uint64_t);
+        static_assert(kBars <= 32, "a lane per barrier");
+        const bool per_warp = lane < 2 || lane == kFree || (lane >= kP && lane < kP + 2 * kPParts);   // a group's four warps arrive
+        if (lane < kBars) mbar_init(smem_u32(ctl) + lane * 8, per_warp ? 4 : 1);
+        if (lane == 0) ctl->abort = 0;
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
+        tmem_relinquish();
+    }
+    grid_dependency_wait();
+    const int kvh = blockIdx.x % p.n_kv_heads;
+    const int per_tile = kRows / p.group;               // new tokens of a tile
+    Job job;
+    const bool any = find_job(p, per_tile, per_cta, blockIdx.x / p.n_kv_heads, lane, job);
+    // Keys that some row of the CTA sees, and the key tiles they lie in.
+    const bool has_t1 = any && job.two;
+    int lo = 0, hi = 0;
+    if (any) {
+        lo = visible_keys(job.s, job.tile0 * per_tile, p.window).lo;
+        hi = visible_keys(job.s, min(job.s.n_new, (job.tile0 + (has_t1 ? 2 : 1)) * per_tile) - 1, p.window).hi;
+    }
+    const int key00 = lo / kKeys * kKeys;
+    const int n_kv = hi > key00 ? (hi - key00 + kKeys - 1) / kKeys : 0;
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    constexpr uint32_t tmem = 0;                        // all columns are taken: the allocation starts at 0
+    if (*reinterpret_cast<volatile uint32_t*>(&ctl->tmem_base) != tmem) ctl->abort = 1;
+
+    if (warp >= 8) {
+        setmaxnreg_dec<88>();
+        if (warp == kLoaderWarp) {
+            // ------------------------------ loader: a lane per page and piece ------------------------------
+            const int box_rows = min(kKeys, 1 << p.page_shift), n_boxes = kKeys / box_rows;
+            const int box = lane & 7, piece = lane >> 3;
+            const bool mine = box < n_boxes && piece < kPieces;
+            const uint32_t all_boxes = (1u << n_boxes) - 1u;
+            const int32_t* row = p.batch.table + (any ? job.b : 0) * p.batch.table_stride;
+            auto needed = [&](int j) {
+                const int k = key00 + j * kKeys + box * box_rows;
+                return mine && j < n_kv && k < hi && k + box_rows > lo;
+            };
+            auto look_up = [&](int j) { return needed(j) ? row[(key00 + j * kKeys + box * box_rows) >> p.page_shift] : 0; };
+            int page = 0, next_page = look_up(0);
+            bool ok = true, good = false;
+            uint32_t boxes = 0;
+            int issued = 0, cleaned = 0;
+            for (; issued < 2 * n_kv && ok; ++issued) {
+                const int j = issued >> 1, kv = issued & 1, slot = issued % kStages;
+                const int base = key00 + j * kKeys;
+                if (kv == 0) {
+                    page = next_page;
+                    next_page = look_up(j + 1);
+                    const bool wanted = needed(j);
+                    good = wanted && (unsigned)page < (unsigned)p.n_pages;
+                    if (wanted && !good) atomicOr(p.status, (int)kStatusBadPage);
+                    boxes = __ballot_sync(0xffffffffu, good) & 0xFFu;
+                }
+                if (issued >= kStages) {
+                    ok = mbar_wait(smem_u32(&ctl->kv_empty[slot]), ((issued / kStages) & 1) ^ 1u, abort_flag, wait_limit);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                const bool clear = kv == 1 && (base < lo || base + kKeys > hi || boxes != all_boxes);
+                const uint32_t full = smem_u32(&ctl->kv_full[slot]), bar = clear ? smem_u32(&ctl->clean) : full;
+                const uint32_t dst = smem + kSmemRing + slot * kTileBytes;
+                if (lane == 0) {
+                    if (kv == 0) ctl->boxes[j % kBoxRing] = boxes;
+                    mbar_arrive_expect_tx(bar, (uint32_t)__popc(boxes) * kPieces * (uint32_t)box_rows * 128u);
+                }
+                __syncwarp();
+                if (good) {
+                    const int first = (base + box * box_rows) & ((1 << p.page_shift) - 1);
+                    tma_load_5d(dst + piece * kPieceBytes + box * box_rows * 128, kv == 0 ? &p.tm_k : &p.tm_v, bar, 0, first, piece, kvh, page);
+                }
+                if (clear) {
+                    ok = mbar_wait(bar, cleaned & 1, abort_flag, wait_limit);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    ++cleaned;
+                    for (int r = lane >> 3; r < kKeys; r += 4) {
+                        const int key = base + r;
+                        if (key >= lo && key < hi && (boxes >> (r / box_rows) & 1u)) continue;
+#pragma unroll
+                        for (int i = 0; i < kPieces; ++i) st_shared_v4(dst + i * kPieceBytes + r * 128 + (lane & 7) * 16, make_uint4(0, 0, 0, 0));
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full);
+                }
+            }
+            if (!ok) {
+                // Leaving early: let the copies this warp started land first (bounded).
+                volatile uint32_t never = 0;
+                mbar_wait(smem_u32(&ctl->clean), cleaned & 1, &never, 4000000ll);
+                for (int i = max(0, issued - kStages); i < issued; ++i)
+                    mbar_wait(smem_u32(&ctl->kv_full[i % kStages]), (i / kStages) & 1, &never, 40000000ll);
+            }
+        } else if (warp == kMmaWarp) {
+            // ------------------------------ MMA issuer, converged ------------------------------
+            constexpr uint32_t idesc_s = umma_idesc_16(kRows, kKeys, false, kFormat), idesc_o = umma_idesc_16(kRows, D, true, kFormat);
+            bool ok = true;
+            const uint64_t q0_desc = umma_smem_desc(smem + kSmemQ, 16, 1024), q1_desc = umma_smem_desc(smem + kSmemQ + kTileBytes, 16, 1024);
+            const uint64_t k_desc0 = umma_smem_desc(smem + kSmemRing, 16, 1024), v_desc0 = umma_smem_desc(smem + kSmemRing, kPieceBytes, 1024);
+            const uint32_t bar_full0 = smem_u32(&ctl->kv_full[0]), bar_empty0 = smem_u32(&ctl->kv_empty[0]), bar_free = smem_u32(&ctl->s_free);
+            // Ring slot of K_j is 2j, of V_j is 2j+1. Every wait is looked at ahead, in front of the MMAs before it.
+            auto slot_off16 = [&](int n) { return (uint32_t)(n % kStages) * (kTileBytes >> 4); };
+            const WarpBarriers bars{abort_flag, wait_limit};
+            auto peek = [&](auto... bar_and_parity) { return look_at(bars, bar_and_parity...); };
+            auto finish = [&](const Look& l) { return f2k::finish(bars, l); };
+            auto bar_full = [&](int n) { return bar_full0 + (n % kStages) * 8; };
+            auto par_full = [&](int n) { return (uint32_t)(n / kStages) & 1u; };
+            auto release = [&](int n) { umma_commit(bar_empty0 + (n % kStages) * 8); };
+            auto bar_p = [&](int t, int part) { return smem_u32(&ctl->p_full[t][part]); };
+            auto issue_s = [&](int t, int j) {
+                tc_fence_after_sync();
+                const uint64_t q = t == 0 ? q0_desc : q1_desc, k = k_desc0 + slot_off16(2 * j);
+                if constexpr (kPieces == 2) umma_ss_x8(tmem + kColS, q, k, idesc_s);
+                else umma_ss_x4(tmem + kColS, q, k, idesc_s);
+                umma_commit(smem_u32(&ctl->s_full[t]));
+            };
+            // O_t (+)= P_t V_j, half by half as the softmax group hands P over; `next` takes the look at what follows.
+            auto issue_pv = [&](int t, int j, const Look& first, auto&& next) -> bool {
+                const uint32_t d = tmem + (t == 0 ? kColO0 : kColO1), a = tmem + (t == 0 ? kColP0 : kColP1);
+                const uint64_t v = v_desc0 + slot_off16(2 * j + 1);
+                if (!finish(first)) return false;
+                const Look half = peek(bar_p(t, 1), (uint32_t)j & 1u);
+                tc_fence_after_sync();
+                umma_ts_x4(d, a, v, idesc_o, j > 0 ? 1u : 0u);
+                if (!finish(half)) return false;
+                next();
+                tc_fence_after_sync();
+                umma_ts_x4(d, a + 32, v + 4 * (2048 >> 4), idesc_o, 1u);
+                umma_commit(smem_u32(&ctl->pv_done[t]));
+                return true;
+            };
+            // With two tiles S0_j is use 2j of the S buffer and S1_j use 2j + 1, with one S0_j is use j; use u waits for
+            // release u - 1.
+            Look look_s{}, look_p{};
+            if (n_kv > 0) {
+                ok = bars.wait(bar_full(0), par_full(0)) && bars.wait(smem_u32(&ctl->q_full[0]), 0);
+                if (ok) issue_s(0, 0);
+                if (ok && has_t1) ok = bars.wait(smem_u32(&ctl->q_full[1]), 0);
+                look_s = peek(bar_free, 0u);
+            }
+            for (int j = 0; j < n_kv && ok; ++j) {
+                if (has_t1) {
+                    if (!(ok = finish(look_s))) break;
+                    if (j > 0) look_p = peek(bar_p(1, 0), (uint32_t)(j - 1) & 1u);
+                    issue_s(1, j);
+                }
+                release(2 * j);
+                auto look_next_s0 = [&] {
+                    if (j + 1 < n_kv)
+                        look_s = peek(bar_full(2 * j + 2), par_full(2 * j + 2), bar_free, has_t1 ? 1u : (uint32_t)(j & 1));
+                };
+                if (has_t1 && j > 0) {
+                    if (!(ok = issue_pv(1, j - 1, look_p, look_next_s0))) break;
+                    release(2 * j - 1);
+                } else {
+                    look_next_s0();
+                }
+                if (j + 1 < n_kv) {
+                    if (!(ok = finish(look_s))) break;
+                }
+                look_p = peek(bar_full(2 * j + 1), par_full(2 * j + 1), bar_p(0, 0), (uint32_t)j & 1u);
+                if (j + 1 < n_kv) issue_s(0, j + 1);
+                if (!(ok = issue_pv(0, j, look_p, [&] { if (has_t1) look_s = peek(bar_free, 0u); }))) break;
+                if (!has_t1) release(2 * j + 1);
+            }
+            if (ok && n_kv > 0 && has_t1) {
+                ok = issue_pv(1, n_kv - 1, peek(bar_p(1, 0), (uint32_t)(n_kv - 1) & 1u), [] {});
+                if (ok) release(2 * n_kv - 1);
+            }
+            if (!ok) {
+                // Leaving early: until the MMAs already issued retire (bounded), so tensor memory is idle when freed.
+                volatile uint32_t never = 0;
+                __syncwarp();
+                umma_commit(smem_u32(&ctl->drain));
+                mbar_wait(smem_u32(&ctl->drain), 0, &never, 40000000ll);
+            }
+        }
+    } else if ((warp < 4 && any) || has_t1) {
+        // ------------------------------ softmax of tile 0 / 1 ------------------------------
+        setmaxnreg_inc<208>();
+        const int t = warp >> 2;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + lane_base + kColS, tP = tmem + lane_base + (t == 0 ? kColP0 : kColP1);
+        const uint32_t tO = tmem + lane_base + (t == 0 ? kColO0 : kColO1);
+        const float c = p.scale_log2;
+        const int tok0 = (job.tile0 + t) * per_tile, rows = min(per_tile, job.s.n_new - tok0) * p.group;
+        constexpr int kChunks = D / 8;                  // 16-byte chunks of a row
+        const uint32_t q_tile = smem + kSmemQ + t * kTileBytes;
+        {   // Q rows to shared memory as the MMA reads them: 128-byte pieces, chunks swizzled by row
+            const int tid = threadIdx.x & 127;
+            const T* q = static_cast<const T*>(p.q) + (long long)(job.s.first + tok0) * p.q_stride + (long long)kvh * p.group * D;
+#pragma unroll 4
+            for (int i = tid; i < kRows * kChunks; i += 128) {
+                const int r = i / kChunks, ch = i % kChunks, tok = r / p.group;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < rows) v = *reinterpret_cast<const uint4*>(q + tok * p.q_stride + (r - tok * p.group) * D + ch * 8);
+                st_shared_v4(q_tile + (ch >> 3) * kPieceBytes + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl->q_full[t]));
+        }
+        const int r = (warp & 3) * 32 + lane;
+        KeyRange see{0, 0};                             // of this thread's row
+        if (r < rows) see = visible_keys(job.s, tok0 + r / p.group, p.window);
+        float m_ref = -INFINITY, l_sum = 0.0f;
+        bool ok = true;
+        const uint32_t all_boxes = (1u << (kKeys / min(kKeys, 1 << p.page_shift))) - 1u;
+
+        for (int j = 0; j < n_kv; ++j) {
+            ok = mbar_wait(smem_u32(&ctl->s_full[t]), j & 1, abort_flag, wait_limit);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const int base = key00 + j * kKeys;
+            const uint32_t boxes = *reinterpret_cast<volatile uint32_t*>(&ctl->boxes[j % kBoxRing]);
+            const bool masked = __any_sync(0xffffffffu, base < see.lo || base + kKeys > see.hi) || boxes != all_boxes;
+            uint32_t s[128];
+            float mx[kMaxChains];
+            auto hide = [&](int from) {                 // scores [from, from + 64) of keys that the row does not see
+                const int first = see.lo - base, end = see.hi - base;
+#pragma unroll
+                for (int i = from; i < from + 64; ++i)
+                    if (i < first || i >= end) s[i] = __float_as_uint(-INFINITY);
+                if (boxes != all_boxes) {
+#pragma unroll
+                    for (int i = from; i < from + 64; i += 16)
+                        if (!(boxes >> (i >> min(p.page_shift, 7)) & 1u)) {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) s[i + k] = __float_as_uint(-INFINITY);
+                        }
+                }
+            };
+            {
+                uint32_t(&s0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[0]);
+                uint32_t(&s1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32]);
+                uint32_t(&s2)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[64]);
+                uint32_t(&s3)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[96]);
+                tmem_ld_x32(tS + 0, s0);
+                tmem_ld_x32(tS + 32, s1);
+                tmem_wait_ld();
+                tmem_ld_x32(tS + 64, s2);
+                tmem_ld_x32(tS + 96, s3);
+                if (masked) hide(0);
+                row_max64<true>(&s[0], mx);
+                tmem_wait_ld();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->s_free));
+            }
+            if (masked) hide(64);
+            row_max64<false>(&s[64], mx);
+            const float m_tile = row_max_finish(mx);
+            const bool pv_seen = j == 0 || mbar_test(smem_u32(&ctl->pv_done[t]), (j - 1) & 1);
+
+            const bool need = (m_tile - m_ref) * c > kLazyThreshold;
+            if (__any_sync(0xffffffffu, need)) {
+                const float m_new = fmaxf(m_ref, m_tile);
+                const float f = m_new == -INFINITY ? 1.0f : ex2_approx((m_ref - m_new) * c);
+                l_sum *= f;
+                m_ref = m_new;
+                if (j > 0) {
+                    ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (j - 1) & 1, abort_flag, wait_limit);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int q = 0; q < D / 32; ++q) {
+                        uint32_t o[32];
+                        tmem_ld_x32(tO + q * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st_x32(tO + q * 32, o);
+                    }
+                }
+            }
+            // A row that has seen no key yet has the reference 0: its weights are 2^-inf = 0.
+            const float neg_mc = m_ref == -INFINITY ? 0.0f : -m_ref * c;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            int pending = -1;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t pk[16];
+                exp_chunk<T>(&s[q * 32], pk, c, neg_mc, sum);
+                if (pending >= 0) {
+                    tmem_wait_st();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&ctl->p_full[t][0]) + pending * 8);
+                    pending = -1;
+                }
+                exp_chunk<T>(&s[q * 32 + 16], pk + 8, c, neg_mc, sum);
+                if (q == 0 && !__all_sync(0xffffffffu, pv_seen)) {
+                    ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (j - 1) & 1, abort_flag, wait_limit);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                if (q == 0) tc_fence_after_sync();
+                tmem_st_x16(tP + q * 16, pk);
+                if ((q + 1) % (4 / kPParts) == 0) pending = (q + 1) / (4 / kPParts) - 1;
+            }
+            if (!ok) break;
+            tmem_wait_st();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl->p_full[t][kPParts - 1]));
+            l_sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+
+        // ------------------------------ epilogue ------------------------------
+        if (ok && n_kv > 0) {
+            ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (n_kv - 1) & 1, abort_flag, wait_limit);
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        if (ok) {
+            tc_fence_after_sync();
+            const bool none = l_sum == 0.0f && m_ref == -INFINITY;      // a row that sees no key is zero
+            const float inv = 1.0f / l_sum;
+            // Rows go out through the shared memory of the tile's Q (no MMA reads it any more), chunk c of row r at
+            // position c ^ (r mod chunks), so that a row leaves in whole lines.
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+                uint32_t o[32];
+                if (n_kv > 0) {
+                    tmem_ld_x32(tO + q * 32, o);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    uint4 v;
+                    v.x = Half16<T>::pack(__uint_as_float(o[i + 0]) * inv, __uint_as_float(o[i + 1]) * inv);
+                    v.y = Half16<T>::pack(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                    v.z = Half16<T>::pack(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+                    v.w = Half16<T>::pack(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                    if (none) v = make_uint4(0, 0, 0, 0);
+                    const int ch = q * 4 + (i >> 3);
+                    st_shared_v4(q_tile + r * (D * 2) + ((ch ^ (r & (kChunks - 1))) << 4), v);
+                }
+            }
+            if (p.lse != nullptr && r < rows) {
+                const int tok = r / p.group;
+                p.lse[(long long)(job.s.first + tok0 + tok) * p.n_heads + kvh * p.group + (r - tok * p.group)] =
+                    none ? -INFINITY : (m_ref * c + log2f(l_sum)) * 0.69314718055994531f;
+            }
+            __syncwarp();
+            constexpr int kRowsAtOnce = 32 / kChunks;
+            const int ch = lane % kChunks;
+            T* out = static_cast<T*>(p.o) + (long long)(job.s.first + tok0) * p.o_stride + (long long)kvh * p.group * D + ch * 8;
+#pragma unroll 4
+            for (int i = lane / kChunks; i < 32; i += kRowsAtOnce) {
+                const int row = (warp & 3) * 32 + i;
+                if (row >= rows) break;
+                const int tok = row / p.group;
+                *reinterpret_cast<uint4*>(out + tok * p.o_stride + (row - tok * p.group) * D) =
+                    ld_shared_v4(q_tile + row * (D * 2) + ((ch ^ (row & (kChunks - 1))) << 4));
+            }
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag != 0u) atomicOr(p.status, (int)kStatusWaitExpired);
+    if (warp == kMmaWarp) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+template <int D>
+constexpr int smem_bytes() { return (2 + kStages) * (D / 64) * (int)kPieceBytes + 1024; }
+
+template <class F>
+cudaError_t with_types(PagedType type, int head_dim, F&& f) {
+    auto by_dim = [&](auto t) { return head_dim == 64 ? f(t, std::integral_constant<int, 64>{}) : f(t, std::integral_constant<int, 128>{}); };
+    return type == kBf16 ? by_dim(__nv_bfloat16{}) : by_dim(__half{});
+}
+
+}  // namespace
+
+cudaError_t paged_prompt_prepare(PagedType type, int head_dim) {
+    return with_types(type, head_dim, [](auto t, auto d) {
+        return cudaFuncSetAttribute(paged_prompt_kernel<decltype(t), decltype(d)::value>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    smem_bytes<decltype(d)::value>());
+    });
+}
+
+cudaError_t paged_prompt_launch(const AttendParams& p, PagedType type, int head_dim, int max_new, int sms, cudaStream_t stream) {
+    return with_types(type, head_dim, [&](auto t, auto d) {
+        // CTAs that the sequences can need: their tiles rounded up, whatever the lengths.
+        const int per_tile = kRows / p.group;
+        auto ctas = [&](int per_cta) {
+            const long long step = (long long)per_tile * per_cta;
+            const long long by_tokens = p.batch.n_tokens / step + p.batch.n_seqs, by_most = (max_new + step - 1) / step * p.batch.n_seqs;
+            return (by_tokens < by_most ? by_tokens : by_most) * p.n_kv_heads;
+        };
+        const int per_cta = ctas(2) >= sms ? 2 : 1;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)ctas(per_cta));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem_bytes<decltype(d)::value>();
+        cfg.stream = stream;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, paged_prompt_kernel<decltype(t), decltype(d)::value>, p, per_cta);
+    });
+}
+
+}  // namespace f2k

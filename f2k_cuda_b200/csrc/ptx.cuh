@@ -305,6 +305,12 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int m, int n, bool b_mn_m
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// The same for either 16-bit type: format 1 = bf16, 0 = f16, of both operands.
+__host__ __device__ constexpr uint32_t umma_idesc_16(int m, int n, bool b_mn_major, uint32_t format) {
+    return (1u << 4) | (format << 7) | (format << 10) | ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(m >> 4) << 24);
+}
+
 // The issuing warp runs converged and every operand is warp-uniform; one elected lane issues.
 // (A divergent single-lane branch would force the operands out of the uniform datapath and cost
 // tens of cycles per MMA on a warp that shares its scheduler with the softmax warps.)
@@ -340,6 +346,29 @@ __device__ __forceinline__ void umma_ss_x8(uint32_t d_tmem, uint64_t a_desc, uin
         "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, more;\n\t"
         "add.s64 a, %1, 1030;\n\t"
         "add.s64 b, %2, 1030;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, more;\n\t"
+        "}\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc)
+        : "memory");
+}
+// The same over 4 k-steps: one box of 64.
+__device__ __forceinline__ void umma_ss_x4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred pe, fresh, more;\n\t"
+        ".reg .b64 a, b;\n\t"
+        "elect.sync _|pe, 0xffffffff;\n\t"
+        "setp.ne.b32 fresh, 0, 0;\n\t"
+        "setp.eq.b32 more, 0, 0;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, fresh;\n\t"
+        "add.s64 a, %1, 2;\n\t"
+        "add.s64 b, %2, 2;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, more;\n\t"
+        "add.s64 a, %1, 4;\n\t"
+        "add.s64 b, %2, 4;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, more;\n\t"
+        "add.s64 a, %1, 6;\n\t"
+        "add.s64 b, %2, 6;\n\t"
         "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, more;\n\t"
         "}\n"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc)

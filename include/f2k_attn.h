@@ -450,14 +450,13 @@ int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const void* q, const voi
                   const void* gamma_q, const void* gamma_k, const float* cos_table, const float* sin_table,
                   int n_positions, float eps, void* q_out, const f2k_kv_strides* strides, void* stream);
 
-/* Bytes of workspace that f2k_kv_attend needs for a batch of these n_seqs, n_tokens and max_new. Calls
- * whose GPU work may overlap need one each. */
+/* Bytes of workspace that f2k_kv_attend needs for a batch with this max_new (0 for prompts). Calls whose GPU work may overlap need one each. */
 size_t f2k_kv_workspace_bytes(const f2k_kv* h, const f2k_kv_batch* batch);
 
 /* o = softmax(scale q K^T) V over the keys that each token sees; zero for a token that sees none.
  * lse: fp32 [n_tokens][n_heads], the logarithm of the sum of exp(scale q K^T) (-inf for none), or
  * NULL. Tokens of a call do not see values of later tokens, but a value that is not finite can make
- * the outputs of up to 127 tokens before it NaN; what lies in pages beyond kv_lens does not matter. */
+ * the outputs of up to 255 tokens before it NaN; what lies in pages beyond kv_lens does not matter. */
 int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const void* q, void* o, float* lse,
                   const f2k_kv_strides* strides, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -79,6 +79,78 @@ def test_cache_with_tokens_before_heads(dtype, cache):
     p.check_attend()
 
 
+# prompts: tiles of 128 rows, one or two a CTA, behind cached keys or not, sequences without a token among them
+PROMPTS = [([64], [64]), ([128], [128]), ([33], [33]), ([300], [300]), ([129, 0, 65, 1, 256], [129, 7, 65, 200, 256]),
+           ([70, 90], [1000, 90]), ([200, 3], [457, 3])]
+
+
+@pytest.mark.parametrize("news,lens", PROMPTS, ids=[str(i) for i in range(len(PROMPTS))])
+@pytest.mark.parametrize("dtype", [BF, HF], ids=ids)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,page", [(8, 2, 16), (2, 2, 64), (3, 1, 128), (14, 2, 32), (4, 1, 256)])
+def test_prompts(news, lens, dtype, dim, heads, kv_heads, page):
+    p = Problem(news, lens, heads, kv_heads, dim, page, dtype, pad=5, gap=8, seed=sum(lens) + dim + heads)
+    p.o.fill_(9.0)
+    p.attend()
+    p.check_attend()
+    assert (p.o[-5:] == 9.0).all() and (p.lse[-5:] == 7.0).all()
+    assert p.kv.device_status() == 0
+
+
+@pytest.mark.parametrize("window", [1, 50, 128, 300])
+@pytest.mark.parametrize("heads,dim,page", [(4, 128, 16), (2, 64, 128), (12, 128, 64)])
+def test_prompts_with_a_window(window, heads, dim, page):
+    """Pages in front of the window are gone: their entries in the table are outside the cache."""
+    p = Problem([500, 40, 130], [500, 900, 700], heads, 2, dim, page, BF, window=window, seed=window)
+    for b, (n, m) in enumerate(zip(p.news, p.lens)):
+        gone = max(0, m - n + 1 - window) // page
+        p.table[b, :gone] = -1
+    p.attend()
+    assert p.kv.device_status() == 0
+    p.table = p.table.clamp(min=0)                      # any page: the formula masks those keys
+    for pages in (p.k_pages, p.v_pages):
+        pages.nan_to_num_(0.0)
+    p.check_attend()
+
+
+def test_many_prompts_two_tiles_a_cta():
+    p = Problem([700, 513, 650, 40, 0, 333], [700, 513, 1200, 40, 3, 2000], 32, 8, 128, 16, BF, seed=21)
+    p.attend()
+    p.check_attend()
+    p = Problem([700, 513, 650], [700, 513, 1200], 30, 10, 64, 16, HF, seed=22)
+    p.attend()
+    p.check_attend()
+
+
+def test_one_more_head_group_than_rows():
+    p = Problem([2, 5], [100, 300], 100, 1, 64, 16, BF, seed=23)          # 100 query heads a key head: a token a tile
+    p.attend()
+    p.check_attend()
+
+
+def test_prompts_with_fewer_keys_than_tokens():
+    """Tokens at negative positions see nothing: zero, and a report."""
+    p = Problem([200, 300, 70], [200, 300, 70], 4, 2, 128, 16, HF, seed=24)
+    p.lens = [0, 120, 70]
+    p.lens_t.copy_(torch.tensor(p.lens, dtype=torch.int32))
+    p.attend()
+    assert p.kv.device_status() == 32
+    p.check_attend()
+
+
+def test_prompt_with_a_page_outside_the_cache():
+    p = Problem([150], [400], 4, 2, 128, 32, HF, seed=25)
+    whole = [p.keys(0, x) for x in (p.k_pages, p.v_pages)]
+    p.table[0, 3] = 10 ** 6                             # keys 96 .. 127
+    p.attend()
+    assert p.kv.device_status() == 16
+    keep = torch.tensor([j for j in range(400) if not 96 <= j < 128], device="cuda")
+    q = p.q[-1].double().unflatten(0, (2, 2))
+    w = torch.softmax(q @ whole[0][:, keep].mT * p.scale, -1)
+    assert ((w @ whole[1][:, keep]).flatten(0, 1) - p.o[-1].double()).abs().max() < 4 * HALF[HF] * whole[1][:, keep].abs().max()
+    assert torch.isfinite(p.o).all()
+
+
 def test_queries_in_place():
     p = Problem([1, 3, 40], [500, 70, 2000], 8, 2, 128, 16, BF, seed=4)
     q = p.q.clone()
