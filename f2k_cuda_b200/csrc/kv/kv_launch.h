@@ -9,8 +9,9 @@ namespace f2k {
 
 cudaError_t kv_append_launch(const AppendParams& p, PagedType type, PagedType cache, int head_dim, cudaStream_t stream);
 
-// Query rows of a work that the token kernel's variants hold: 16, 32 or 64.
+// Query rows of a work that the token kernel's variants hold: 8, 16, 32 or 64; and the CTAs it runs with.
 int         token_rows(long long rows);
+int         token_ctas(int sms);
 cudaError_t paged_token_prepare(PagedType type, PagedType cache, int head_dim);   // load the kernels on the current device
 // rows: of a tile, one of token_rows(); used_rows: the most that any tile of the call has.
 cudaError_t paged_token_launch(const AttendParams& p, PagedType type, PagedType cache, int head_dim, int rows, int used_rows,

@@ -18,6 +18,13 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
+// An 8 x 8 matrix of 16-bit elements, two to a lane, transposed across the warp.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t w) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+    return r;
+}
+
 template <class T> struct Half16;      // what differs between the 16-bit types
 template <> struct Half16<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {

@@ -4,6 +4,7 @@
 #include "../attn_params.h"
 #include "../handle_device.h"
 #include "kv_launch.h"
+#include "token_work.h"
 
 #include <cmath>
 #include <cstdio>
@@ -97,9 +98,9 @@ struct Workspace {
 Workspace workspace_of(const f2k_kv* h, int rows) {
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     Workspace w;
-    const size_t shares = 2 * (size_t)h->sms;
+    const size_t ctas = token_ctas(h->sms), shares = 2 * ctas;
     w.join = 0;
-    w.ml = up(sizeof(int4) * h->sms);
+    w.ml = up(sizeof(int4) * ctas);
     w.o = w.ml + up(shares * rows * sizeof(float2));
     w.bytes = w.o + shares * rows * h->cfg.head_dim * sizeof(float);
     return w;
@@ -256,13 +257,13 @@ int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const void* q, void* o, 
     const int unit = token_unit_keys(c.head_dim * (c.cache_type == F2K_E4M3 ? 1 : 2));
     const long long keys = (long long)batch->table_width << h->page_shift;
     const double tiles = (double)batch->n_tokens * p.group / rows + batch->n_seqs;
-    if (tiles * c.n_kv_heads * (double)(keys / unit + 1) >= 4294967295.0)
+    if (tiles * c.n_kv_heads * (double)(keys / unit + 1 + kWorkCost) >= 4294967295.0)
         return fail(h, F2K_ERR_UNSUPPORTED, "the batch could hold 2^32 pieces of work: make two calls of it");
     uint8_t* w = static_cast<uint8_t*>(workspace);
     p.ws_join = reinterpret_cast<int4*>(w + ws.join);
     p.ws_ml = reinterpret_cast<float2*>(w + ws.ml);
     p.ws_o = reinterpret_cast<float*>(w + ws.o);
-    p.n_ctas = h->sms;
+    p.n_ctas = token_ctas(h->sms);
     p.tm_k = h->token_k;
     p.tm_v = h->token_v;
     const long long used = (long long)batch->max_new * p.group;

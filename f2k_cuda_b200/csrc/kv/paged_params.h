@@ -78,11 +78,11 @@ F2K_HD SeqWork seq_work(const SeqView& s, int group, int rows, int unit, int win
     w.n_units = n > 1 ? n : 1;
     return w;
 }
-// Units that CTA c of n takes: [first, next).
+// First place of the line that CTA c of n takes.
 F2K_HD unsigned piece_begin(unsigned total, int n, int c) {
     return (unsigned)((unsigned long long)total * (unsigned)c / (unsigned)n);
 }
-// CTAs that get units: no more than give each `least`, so that a short batch is not cut finer than it pays.
+// CTAs that get places: no more than give each `least`, so that a short batch is not cut finer than it pays.
 F2K_HD int pieces(unsigned total, int n_ctas, int least) {
     const unsigned want = total / (unsigned)least;
     return want < 1 ? 1 : (want > (unsigned)n_ctas ? n_ctas : (int)want);

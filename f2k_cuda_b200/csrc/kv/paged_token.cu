@@ -7,15 +7,18 @@
 //    piece of it (token_work.h), so ragged lengths cost nothing and one long sequence spreads over the GPU. A work
 //    that a cut goes through is left as unnormalised rows with their maxima and sums, one set per piece, and a
 //    second kernel joins the sets in the order of the keys; a whole work is written by the CTA that has it.
-//  * A CTA is eight warps, one per SM. RW warps share the rows (16 each), and the KW = 8 / RW groups of them take every
-//    KW-th unit. A group has a ring of K and V boxes of its own, fetched by TMA (one lane of the group's first warp),
-//    192 KB per SM in flight or in use, and no group waits for another before the end of a work.
-//  * S = Q K^T and O += P V are m16n8k16 products of the warp with the softmax on their registers: 16 rows are enough
-//    for `group` heads, where a tcgen05 tile would have 128, and the row of a 16-key unit is read by ldmatrix once.
+//  * A CTA is four warps, two CTAs per SM: one reads while the other begins or ends a work. RW warps share the rows, and the
+//    KW = 4 / RW groups of them take every KW-th unit. A group has a ring of K and V boxes of its own, fetched by TMA (one
+//    lane of the group's first warp), and no group waits for another before the end of a work.
+//  * Keys are the long side of the products: S^T = K Q^T and O^T += V^T P^T as m16n8k16 products of the warp, K and V the
+//    16-row operands straight from ldmatrix, eight query rows a column tile. Eight rows hold the heads of most models'
+//    groups; a tcgen05 tile would have 128. With rows as the 16-row operand half of every product, register and
+//    exponential was spent on rows that do not exist (96 sequences of about 2700 keys, e4m3, 40 heads over 8: 193 us).
 //
-// Online softmax per warp: maximum, sum and O in fp32, exponents of 2; P is rounded to 16 bits for P V, the sum is
-// taken before. Rows are masked by key number; values of keys that no row of the tile sees are cleared in registers, so
-// what lies in the rest of a page (NaN included) does not matter.
+// Online softmax per warp, raw scores, exponents of 2, fp32; a row's reference only moves when a score exceeds it by 2^8, so
+// most units need no maximum across lanes. P is rounded to 16 bits for the product, the sum is taken before. Rows
+// are masked by key number; values of keys that no row of the tile sees are cleared in registers, so what lies in the
+// rest of a page (NaN included) does not matter.
 //
 // e4m3 caches: the bytes become fp16 in registers (exactly), the products are fp16 ones. A thread's four bytes of K are
 // neighbours in head_dim; a contraction may be taken in any order, so Q is laid out to match. bf16 queries are brought
@@ -34,47 +37,54 @@ using namespace f2k::ptx;
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kStagesAll = 24;                 // over the groups of a CTA
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kCtasPerSm = 2;
+constexpr uint32_t kRingBytes = 96 * 1024;     // over the groups of a CTA
+constexpr int kMostStages = 24;
+constexpr int kSeqsHeld = kThreads;            // sequences kept in shared memory; larger batches are looked up where they lie
+constexpr float kLazyThreshold = 8.0f;         // log2 units
 
-template <bool kE4m3, int D, int RW>
+// NT tiles of eight rows a warp, RW warps over the rows.
+template <bool kE4m3, int D, int NT, int RW>
 struct Shape {
-    static constexpr int kRows = 16 * RW, KW = kWarps / RW;
+    static constexpr int kRows = 8 * NT * RW, KW = kWarps / RW;
     static constexpr int kRowBytes = D * (kE4m3 ? 1 : 2);
     static constexpr int kUnit = token_unit_keys(kRowBytes);
     static constexpr int kPiece = kRowBytes < 128 ? kRowBytes : 128;     // bytes of a shared-memory row
     static constexpr uint32_t kTile = kUnit * kRowBytes, kStage = 2 * kTile;   // K or V of a unit; both
-    static constexpr int kRing = kStagesAll / KW;
-    static constexpr int kSlots = kWarps / 2;
-    static constexpr uint32_t kSlotFloats = 16 * D;
-    static constexpr uint32_t kSmem = kStagesAll * kStage + kSlots * kSlotFloats * 4;
+    static constexpr int kStages = kRingBytes / kStage, kRing = kStages / KW;
+    static_assert(kStages <= kMostStages && kRing >= 3, "stages");
+    static constexpr int kSlice = D / 16 / KW;                            // 16-row tiles of O^T that a warp sums up and writes
+    static constexpr int kSliceFloats = kSlice * 16 * 8;
+    static constexpr uint32_t kSlots = kWarps * (KW - 1) * kSliceFloats;  // floats: every warp's other slices, one row tile
+    static constexpr uint32_t kSmem = kRingBytes + kSlots * 4;
 };
 
 struct Ctl {
-    uint64_t full[kStagesAll], empty[kStagesAll];
-    uint32_t boxes[kStagesAll];                // which boxes of the stage hold keys
-    float2 ml[kWarps][16];
+    uint64_t full[kMostStages], empty[kMostStages];
+    uint32_t boxes[kMostStages];               // which boxes of the stage hold keys
+    float2 ml[kWarps][32];
     unsigned scan[kWarps];
-    unsigned total, seq_begin;
+    unsigned seq_begin;
     int seq;
     uint32_t abort;
+    int first[kSeqsHeld], n_new[kSeqsHeld], len[kSeqsHeld];
 };
 
-template <class T, bool kE4m3, int D, int RW>
-__global__ void __launch_bounds__(kThreads, 1)
+template <class T, bool kE4m3, int D, int NT, int RW>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
 paged_token_kernel(const __grid_constant__ AttendParams p) {
-    using S = Shape<kE4m3, D, RW>;
+    using S = Shape<kE4m3, D, NT, RW>;
     using M = std::conditional_t<kE4m3, __half, T>;          // the type of the products
-    constexpr int KW = S::KW, kUnit = S::kUnit, kRing = S::kRing, kSteps = D / 16;
+    constexpr int KW = S::KW, kUnit = S::kUnit, kRing = S::kRing, kSteps = D / 16, kBlocks = kUnit / 16;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Ctl ctl;
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    float* slots = reinterpret_cast<float*>(smem_raw + (smem - smem_u32(smem_raw)) + kStagesAll * S::kStage);
+    float* slots = reinterpret_cast<float*>(smem_raw + (smem - smem_u32(smem_raw)) + kRingBytes);
     volatile uint32_t* abort_flag = &ctl.abort;
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int kw = warp / RW, rw = warp % RW;
-    if (threadIdx.x < kStagesAll) {
+    if (threadIdx.x < kMostStages) {
         mbar_init(smem_u32(&ctl.full[threadIdx.x]), 1);
         mbar_init(smem_u32(&ctl.empty[threadIdx.x]), RW);
     }
@@ -85,15 +95,18 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
     grid_dependency_wait();
 
     // ---- where this CTA's piece of the line lies: a sum over the sequences, a run of them per thread
+    const bool held = p.batch.n_seqs <= kSeqsHeld;
+    auto seq = [&](int b) {
+        return held ? SeqView{ctl.first[b], ctl.n_new[b], ctl.len[b], false} : seq_of(p.batch, p.page_shift, b);
+    };
     const int per = (p.batch.n_seqs + kThreads - 1) / kThreads;
     const int b_first = min(p.batch.n_seqs, (int)threadIdx.x * per), b_last = min(p.batch.n_seqs, b_first + per);
     unsigned mine = 0;
     for (int b = b_first; b < b_last; ++b) {
-        Where x;
-        x.b = b;
-        load_seq(p, S::kRows, kUnit, x);
-        if (x.s.bad) atomicOr(p.status, (int)kStatusBadLength);
-        mine += seq_units(p, x.w);
+        const SeqView s = seq_of(p.batch, p.page_shift, b);
+        if (s.bad) atomicOr(p.status, (int)kStatusBadLength);
+        if (held) ctl.first[b] = s.first, ctl.n_new[b] = s.n_new, ctl.len[b] = s.len;
+        mine += seq_places(p, seq_work(s, p.group, S::kRows, kUnit, p.window));
     }
     unsigned upto = mine;
 #pragma unroll
@@ -109,7 +122,7 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
         if (w < warp) upto += ctl.scan[w];
         total += ctl.scan[w];
     }
-    const int n_pieces = pieces(total, p.n_ctas, KW);
+    const int n_pieces = pieces(total, p.n_ctas, kWorkCost + KW);
     const int cta = blockIdx.x;
     if (cta >= n_pieces || total == 0) {
         if (threadIdx.x == 0) p.ws_join[cta] = make_int4(0, 0, 0, 0);
@@ -119,15 +132,13 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
     if (begin >= upto - mine && begin < upto) {
         unsigned at = upto - mine;
         for (int b = b_first;; ++b) {
-            Where x;
-            x.b = b;
-            load_seq(p, S::kRows, kUnit, x);
-            if (begin - at < seq_units(p, x.w)) {
+            const unsigned places = seq_places(p, seq_work(seq(b), p.group, S::kRows, kUnit, p.window));
+            if (begin - at < places) {
                 ctl.seq = b;
                 ctl.seq_begin = at;
                 break;
             }
-            at += seq_units(p, x.w);
+            at += places;
         }
     }
     __syncthreads();
@@ -137,7 +148,8 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
     Where start;
     start.b = ctl.seq;
     start.seq_begin = ctl.seq_begin;
-    load_seq(p, S::kRows, kUnit, start);
+    start.s = seq(start.b);
+    start.w = seq_work(start.s, p.group, S::kRows, kUnit, p.window);
     const uint32_t ring = smem + kw * kRing * S::kStage;
     const uint32_t full0 = smem_u32(&ctl.full[kw * kRing]), empty0 = smem_u32(&ctl.empty[kw * kRing]);
     const int box_rows = min(kUnit, 1 << p.page_shift);      // 16, or 32
@@ -184,59 +196,56 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
             }
         }
         ++fetched;
-        ahead.next(p);
+        ahead.next(p, seq);
         look_up();
     };
     if (rw == 0) {
         ahead.x = start;
         ahead.end = end;
         ahead.kw = kw;
-        ahead.enter(p, begin);
+        ahead.enter(p, seq, begin);
         look_up();
         for (int i = 0; i < kRing - 1; ++i) fetch();
     }
 
     // ---- work by work
-    const int g8 = lane >> 2, t4 = lane & 3;                  // fragment row and column group
+    const int g8 = lane >> 2, t4 = lane & 3;                  // rows g8 of an operand's column tile; 2 t4, 2 t4 + 1 of a result's
     int used = 0;                                             // units of the group consumed
     Walk walk;
     walk.x = start;
     walk.end = end;
     walk.kw = kw;
-    for (unsigned at = begin; at < end;) {
-        find_work(p, S::kRows, kUnit, at, walk.x);
-        const Where x = walk.x;
-        const unsigned work_end = x.work_begin + (unsigned)x.w.n_units;
-        walk.work_end = min(end, work_end);
-        walk.u = at + (unsigned)kw;
-        const int tile_rows = min(S::kRows, x.s.n_new * p.group - x.rt * S::kRows);
-        const bool active = rw * 16 < tile_rows;
+    for (unsigned at = begin; at < end; at = walk.stop) {
+        const bool any = walk.begin(p, seq, at);
+        const Where& x = walk.x;
         if (at == begin && threadIdx.x == 0) p.ws_join[cta] = make_int4(x.b, x.kvh, x.rt, shares_to_join(x, total, n_pieces, cta));
+        if (!any) break;                                      // the piece ends before the work's first unit
+        const int tile_rows = min(S::kRows, x.s.n_new * p.group - x.rt * S::kRows);
+        const bool active = rw * 8 * NT < tile_rows;
 
-        // rows of this thread: rw * 16 + g8 and + 8
-        KeyRange see[2];
-        float coef[2];
-        uint32_t qa[kSteps][4];
+        // ---- Q: row n of column tile nt is the tile's row rw * 8 NT + 8 nt + n
+        uint32_t qb[NT][kSteps][2];
+        float coef[NT][2];
+        KeyRange see[NT][2];
+        const float scale = kE4m3 && p.k_scale ? p.scale_log2 * p.k_scale[x.kvh] : p.scale_log2;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = x.rt * S::kRows + rw * 16 + g8 + 8 * h;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = x.rt * S::kRows + rw * 8 * NT + nt * 8 + g8;
             const int tok = r / p.group, head = x.kvh * p.group + (r - tok * p.group);
             const bool valid = tok < x.s.n_new;
-            see[h] = valid ? visible_keys(x.s, tok, p.window) : KeyRange{0, 0};
             const T* row = static_cast<const T*>(p.q) + (x.s.first + tok) * p.q_stride + (long long)head * D;
-            coef[h] = p.scale_log2;
+            coef[nt][0] = coef[nt][1] = scale;
             if constexpr (!kE4m3) {
 #pragma unroll
                 for (int ks = 0; ks < kSteps; ++ks) {
-                    qa[ks][h] = valid ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * t4) : 0u;
-                    qa[ks][2 + h] = valid ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8 + 2 * t4) : 0u;
+                    qb[nt][ks][0] = valid ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * t4) : 0u;
+                    qb[nt][ks][1] = valid ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8 + 2 * t4) : 0u;
                 }
             } else {
                 uint2 raw[kSteps];
 #pragma unroll
                 for (int ks = 0; ks < kSteps; ++ks)
                     raw[ks] = valid ? *reinterpret_cast<const uint2*>(row + ks * 16 + 4 * t4) : make_uint2(0u, 0u);
-                if (p.k_scale) coef[h] *= p.k_scale[x.kvh];
                 if constexpr (std::is_same_v<T, __nv_bfloat16>) {
                     float top = 0.f;
 #pragma unroll
@@ -248,25 +257,34 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
                     // largest element into [2^14, 2^15); an infinite one is left as it is
                     const unsigned e = __float_as_uint(top) >> 23;
                     const unsigned f = e == 255u ? 127u : min(253u, 268u - e);
-                    const float up = __uint_as_float(f << 23);
-                    coef[h] *= __uint_as_float((254u - f) << 23);
+                    const float up = __uint_as_float(f << 23), down = __uint_as_float((254u - f) << 23);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) coef[nt][h] *= __shfl_sync(0xffffffffu, down, (2 * t4 + h) * 4);
 #pragma unroll
                     for (int ks = 0; ks < kSteps; ++ks) {
-                        qa[ks][h] = Half16<M>::pack(Half16<T>::lo(raw[ks].x) * up, Half16<T>::hi(raw[ks].x) * up);
-                        qa[ks][2 + h] = Half16<M>::pack(Half16<T>::lo(raw[ks].y) * up, Half16<T>::hi(raw[ks].y) * up);
+                        qb[nt][ks][0] = Half16<M>::pack(Half16<T>::lo(raw[ks].x) * up, Half16<T>::hi(raw[ks].x) * up);
+                        qb[nt][ks][1] = Half16<M>::pack(Half16<T>::lo(raw[ks].y) * up, Half16<T>::hi(raw[ks].y) * up);
                     }
                 } else {
 #pragma unroll
-                    for (int ks = 0; ks < kSteps; ++ks) qa[ks][h] = raw[ks].x, qa[ks][2 + h] = raw[ks].y;
+                    for (int ks = 0; ks < kSteps; ++ks) qb[nt][ks][0] = raw[ks].x, qb[nt][ks][1] = raw[ks].y;
                 }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int i = (x.rt * S::kRows + rw * 8 * NT + nt * 8 + 2 * t4 + h) / p.group;
+                see[nt][h] = i < x.s.n_new ? visible_keys(x.s, i, p.window) : KeyRange{0, 0};
             }
         }
 
-        float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float o[NT][kSteps][4], m[NT][2], l[NT][2];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+            for (int i = 0; i < kSteps; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        }
         // rows see keys [lo_all, hi_all) without exception
         const int i_first = x.rt * S::kRows / p.group, i_last = min(x.s.n_new - 1, (x.rt * S::kRows + S::kRows - 1) / p.group);
         const int lo_all = visible_keys(x.s, i_last, p.window).lo, hi_all = visible_keys(x.s, i_first, p.window).hi;
@@ -291,84 +309,101 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
                     const int twist = kChunks == 8 ? (r & 7) : ((r >> 1) & 3);
                     return tile + box * box_bytes + (piece * box_rows + r) * S::kPiece + ((c ^ twist) << 4);
                 };
-                float s[kUnit / 8][4];
+                float s[NT][kBlocks][4];
 #pragma unroll
-                for (int i = 0; i < kUnit / 8; ++i)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-                // ---- S = Q K^T
+                    for (int kb = 0; kb < kBlocks; ++kb) s[nt][kb][0] = s[nt][kb][1] = s[nt][kb][2] = s[nt][kb][3] = 0.f;
+                // ---- S^T = K Q^T
+                const int key_k = ((lane >> 3 & 1) << 3) + (lane & 7);
+                if constexpr (!kE4m3) {
 #pragma unroll
-                for (int kb = 0; kb < kUnit / 16; ++kb) {
-                    if constexpr (!kE4m3) {
-                        const int key = kb * 16 + ((lane >> 4) << 3) + (lane & 7);
+                    for (int ks = 0; ks < kSteps; ++ks)
 #pragma unroll
-                        for (int ks = 0; ks < kSteps; ++ks) {
-                            uint32_t r[4];
-                            ldmatrix_x4(r, at_smem(tile_k, key, ks * 2 + ((lane >> 3) & 1)));
-                            Half16<M>::mma(s[2 * kb], qa[ks], r[0], r[1]);
-                            Half16<M>::mma(s[2 * kb + 1], qa[ks], r[2], r[3]);
+                        for (int kb = 0; kb < kBlocks; ++kb) {
+                            uint32_t a[4];
+                            ldmatrix_x4(a, at_smem(tile_k, kb * 16 + key_k, ks * 2 + (lane >> 4)));
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) Half16<M>::mma(s[nt][kb], a, qb[nt][ks][0], qb[nt][ks][1]);
                         }
-                    } else {
-                        const int key = kb * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+                } else {
 #pragma unroll
-                        for (int ks = 0; ks < kSteps; ks += 2) {
+                    for (int ks = 0; ks < kSteps; ks += 2)
+#pragma unroll
+                        for (int kb = 0; kb < kBlocks; ++kb) {
                             uint32_t r[4];
-                            ldmatrix_x4(r, at_smem(tile_k, key, ks + (lane >> 4)));
+                            ldmatrix_x4(r, at_smem(tile_k, kb * 16 + key_k, ks + (lane >> 4)));
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                Half16<M>::mma(s[2 * kb + (i & 1)], qa[ks + (i >> 1)], f16x2_of_e4m3x2(r[i]), f16x2_of_e4m3x2(r[i] >> 16));
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t a[4] = {f16x2_of_e4m3x2(r[2 * i]), f16x2_of_e4m3x2(r[2 * i + 1]), f16x2_of_e4m3x2(r[2 * i] >> 16),
+                                                       f16x2_of_e4m3x2(r[2 * i + 1] >> 16)};
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) Half16<M>::mma(s[nt][kb], a, qb[nt][ks + i][0], qb[nt][ks + i][1]);
+                            }
                         }
-                    }
                 }
-                // ---- scale, mask, running maximum
+                // ---- mask, reference maximum
                 const bool whole = key0 >= lo_all && key0 + kUnit <= hi_all && boxes == (1u << n_boxes) - 1u;
-                float top[2] = {-INFINITY, -INFINITY};
+                if (!whole) {
 #pragma unroll
-                for (int i = 0; i < kUnit / 8; ++i)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float v = s[i][j] * coef[j >> 1];
-                        if (!whole) {
-                            const int k = i * 8 + 2 * t4 + (j & 1), key = key0 + k;
-                            const bool in = key >= see[j >> 1].lo && key < see[j >> 1].hi && (boxes >> (k >= box_rows ? 1 : 0) & 1u);
-                            v = in ? v : -INFINITY;
-                        }
-                        s[i][j] = v;
-                        top[j >> 1] = fmaxf(top[j >> 1], v);
-                    }
-                float ref[2];
-                bool moved = false;
+                        for (int kb = 0; kb < kBlocks; ++kb)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-                    moved |= top[h] > m[h];
+                            for (int j = 0; j < 4; ++j) {
+                                const int k = kb * 16 + (j >> 1) * 8 + g8, key = key0 + k;
+                                const KeyRange& r = see[nt][j & 1];
+                                if (!(key >= r.lo && key < r.hi && (boxes >> (k >= box_rows ? 1 : 0) & 1u))) s[nt][kb][j] = -INFINITY;
+                            }
                 }
-                if (__any_sync(0xffffffffu, moved)) {
+                float top[NT][2];
+                bool moves = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float to = fmaxf(m[h], top[h]);
-                        const float f = to == -INFINITY ? 1.f : ex2_approx(m[h] - to);
-                        m[h] = to;
-                        l[h] *= f;
+                        top[nt][h] = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < D / 8; ++i) o[i][2 * h] *= f, o[i][2 * h + 1] *= f;
+                        for (int kb = 0; kb < kBlocks; ++kb) top[nt][h] = fmaxf(top[nt][h], fmaxf(s[nt][kb][h], s[nt][kb][2 + h]));
+                        moves |= (top[nt][h] - m[nt][h]) * coef[nt][h] > kLazyThreshold || (m[nt][h] == -INFINITY && top[nt][h] > -INFINITY);
                     }
-                }
+                if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) ref[h] = m[h] == -INFINITY ? 0.f : m[h];
-                // ---- P, its sum, and O += P V
-#pragma unroll
-                for (int kb = 0; kb < kUnit / 16; ++kb) {
-                    uint32_t pa[4];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float a = ex2_approx(s[2 * kb + i][2 * h] - ref[h]), b = ex2_approx(s[2 * kb + i][2 * h + 1] - ref[h]);
-                            l[h] += a + b;
-                            pa[2 * i + h] = Half16<M>::pack(a, b);
+                            float to = top[nt][h];
+                            to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 4));
+                            to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 8));
+                            to = fmaxf(m[nt][h], fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16)));
+                            const float f = m[nt][h] == to ? 1.f : ex2_approx((m[nt][h] - to) * coef[nt][h]);
+                            m[nt][h] = to;
+                            l[nt][h] *= f;
+#pragma unroll
+                            for (int i = 0; i < kSteps; ++i) o[nt][i][h] *= f, o[nt][i][2 + h] *= f;
                         }
+                }
+                // ---- P^T and its sum
+                uint32_t pb[NT][kBlocks][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float neg[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) neg[h] = m[nt][h] == -INFINITY ? 0.f : -m[nt][h] * coef[nt][h];
+#pragma unroll
+                    for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float a = ex2_approx(fmaf(s[nt][kb][2 * i], coef[nt][0], neg[0]));
+                            const float b = ex2_approx(fmaf(s[nt][kb][2 * i + 1], coef[nt][1], neg[1]));
+                            l[nt][0] += a;
+                            l[nt][1] += b;
+                            pb[nt][kb][i] = movmatrix_trans(Half16<M>::pack(a, b));
+                        }
+                }
+                // ---- O^T += V^T P^T
+#pragma unroll
+                for (int kb = 0; kb < kBlocks; ++kb) {
                     // Values of keys that no row of the tile sees are not read as numbers: they may be anything.
                     uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
                     if (!whole) {
@@ -384,25 +419,28 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
                         }
                     }
                     if constexpr (!kE4m3) {
-                        const int key = kb * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+                        const int key = kb * 16 + (lane >> 4) * 8 + (lane & 7);
 #pragma unroll
-                        for (int dt = 0; dt < D / 16; ++dt) {
-                            uint32_t r[4];
-                            ldmatrix_x4_trans(r, at_smem(tile_v, key, dt * 2 + (lane >> 4)));
-                            Half16<M>::mma(o[2 * dt], pa, r[0] & keep[0], r[1] & keep[1]);
-                            Half16<M>::mma(o[2 * dt + 1], pa, r[2] & keep[0], r[3] & keep[1]);
+                        for (int dt = 0; dt < kSteps; ++dt) {
+                            uint32_t a[4];
+                            ldmatrix_x4_trans(a, at_smem(tile_v, key, dt * 2 + (lane >> 3 & 1)));
+                            if (!whole) a[0] &= keep[0], a[1] &= keep[0], a[2] &= keep[1], a[3] &= keep[1];
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) Half16<M>::mma(o[nt][dt], a, pb[nt][kb][0], pb[nt][kb][1]);
                         }
                     } else {
-                        const int key = kb * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
-                        for (int dt = 0; dt < D / 16; dt += 2) {
+                        for (int dt = 0; dt < kSteps; dt += 2) {
                             uint32_t r[4];
-                            ldmatrix_x4_trans(r, at_smem(tile_v, key, dt + (lane >> 4)));
+                            ldmatrix_x4_trans(r, at_smem(tile_v, kb * 16 + key_k, dt + (lane >> 4)));
+                            if (!whole) r[0] &= keep[0], r[1] &= keep[1], r[2] &= keep[0], r[3] &= keep[1];
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
-                                const uint32_t a = r[2 * i] & keep[0], b = r[2 * i + 1] & keep[1];
-                                Half16<M>::mma(o[2 * (dt + i)], pa, f16x2_of_e4m3x2(__byte_perm(a, 0, 0x4420)), f16x2_of_e4m3x2(__byte_perm(b, 0, 0x4420)));
-                                Half16<M>::mma(o[2 * (dt + i) + 1], pa, f16x2_of_e4m3x2(__byte_perm(a, 0, 0x4431)), f16x2_of_e4m3x2(__byte_perm(b, 0, 0x4431)));
+                                // a word: two keys of two neighbours of head_dim; even ones are rows 0-7 of the tile, odd ones 8-15
+                                const uint32_t a[4] = {f16x2_of_e4m3x2(__byte_perm(r[2 * i], 0, 0x4420)), f16x2_of_e4m3x2(__byte_perm(r[2 * i], 0, 0x4431)),
+                                                       f16x2_of_e4m3x2(__byte_perm(r[2 * i + 1], 0, 0x4420)), f16x2_of_e4m3x2(__byte_perm(r[2 * i + 1], 0, 0x4431))};
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) Half16<M>::mma(o[nt][dt + i], a, pb[nt][kb][0], pb[nt][kb][1]);
                             }
                         }
                     }
@@ -412,90 +450,128 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
             if (RW > 1 && lane == 0) mbar_arrive(empty0 + stage * 8);
         }
 
-        // ---- the groups' shares of the work, joined
+        // ---- the groups' shares of the work: maxima and sums, then row tile by row tile every warp sums a slice of head_dim up
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            if (t4 == 0) ctl.ml[warp][g8 + 8 * h] = make_float2(m[h], l[h]);
-        }
-        constexpr int kHalf = KW / 2;
-        // Four neighbouring columns of a slot's row stand together; 8-column runs are moved by the row against bank conflicts.
-        auto slot_at = [&](int slot, int row, int col) { return slots + slot * S::kSlotFloats + row * D + (col ^ ((row & 7) << 3)); };
-        auto each_pair = [&](auto&& f) {       // f(row, column, value, value) for this thread's elements of O, two neighbours at a time
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if constexpr (kE4m3) {
-                        f(h, c * 16 + 4 * t4, o[2 * c][2 * h], o[2 * c + 1][2 * h]);
-                        f(h, c * 16 + 4 * t4 + 2, o[2 * c][2 * h + 1], o[2 * c + 1][2 * h + 1]);
-                    } else {
-                        f(h, c * 16 + 2 * t4, o[2 * c][2 * h], o[2 * c][2 * h + 1]);
-                        f(h, c * 16 + 8 + 2 * t4, o[2 * c + 1][2 * h], o[2 * c + 1][2 * h + 1]);
-                    }
-                }
-        };
-        if (kw >= kHalf)
-            each_pair([&](int h, int col, float a, float b) {
-                *reinterpret_cast<float2*>(slot_at((kw - kHalf) * RW + rw, g8 + 8 * h, col)) = make_float2(a, b);
-            });
-        __syncthreads();
-        if (*abort_flag != 0u) break;                          // the same in every thread: nobody waits between the barriers
-        if (kw < kHalf) {
-            float mine_f[2], other_f[2];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float all = -INFINITY;
-#pragma unroll
-                for (int k = 0; k < KW; ++k) all = fmaxf(all, ctl.ml[k * RW + rw][g8 + 8 * h].x);
-                const float to = all == -INFINITY ? 0.f : all;
-                mine_f[h] = ex2_approx(m[h] - to);
-                other_f[h] = ex2_approx(ctl.ml[(kw + kHalf) * RW + rw][g8 + 8 * h].x - to);
+                l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], 4);
+                l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], 8);
+                l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], 16);
+                if (m[nt][h] != -INFINITY) m[nt][h] *= coef[nt][h];            // from here on in log2 units
+                if (g8 == 0) ctl.ml[warp][nt * 8 + 2 * t4 + h] = make_float2(m[nt][h], l[nt][h]);
             }
-            each_pair([&](int h, int col, float a, float b) {
-                float2* s2 = reinterpret_cast<float2*>(slot_at(kw * RW + rw, g8 + 8 * h, col));
-                const float2 v = *s2;
-                *s2 = make_float2(a * mine_f[h] + v.x * other_f[h], b * mine_f[h] + v.y * other_f[h]);
-            });
-        }
-        __syncthreads();
-        // ---- rows out: finished, or a piece's share for the join
-        const bool from_start = at == x.work_begin, to_end = walk.work_end == work_end;
+        const bool from_start = at <= x.first_unit(), to_end = walk.stop == x.work_end;
         const int share = share_of(cta, from_start);
         const float v_scale = kE4m3 && p.v_scale ? p.v_scale[x.kvh] : 1.f;
-        for (int idx = threadIdx.x; idx < tile_rows * (D / 4); idx += kThreads) {
-            const int r = idx / (D / 4), col = (idx % (D / 4)) * 4, r16 = r & 15, rwi = r >> 4;
-            float all = -INFINITY, sum = 0.f;
+        bool stopped = false;
 #pragma unroll
-            for (int k = 0; k < KW; ++k) all = fmaxf(all, ctl.ml[k * RW + rwi][r16].x);
-            const float to = all == -INFINITY ? 0.f : all;
+        for (int nt = 0; nt < NT; ++nt) {
+            // slice k of this warp's O^T, in the order of its registers: a float2 a lane
+            auto slot_at = [&](int from_kw, int to_kw, int i, int half) {
+                const int other = to_kw < from_kw ? to_kw : to_kw - 1;
+                return reinterpret_cast<float2*>(slots + ((from_kw * RW + rw) * (KW - 1) + other) * S::kSliceFloats + i * 128 + half * 64) + lane;
+            };
+            if (nt > 0) __syncthreads();
 #pragma unroll
-            for (int k = 0; k < KW; ++k) {
-                const float2 v = ctl.ml[k * RW + rwi][r16];
-                sum += v.y * ex2_approx(v.x - to);
+            for (int k = 0; k < KW; ++k)
+                if (k != kw) {
+#pragma unroll
+                    for (int i = 0; i < S::kSlice; ++i) {
+                        const float(&v)[4] = o[nt][k * S::kSlice + i];
+                        *slot_at(kw, k, i, 0) = make_float2(v[0], v[1]);
+                        *slot_at(kw, k, i, 1) = make_float2(v[2], v[3]);
+                    }
+                }
+            __syncthreads();
+            if (nt == 0) stopped = *abort_flag != 0u;          // the same in every thread: nobody waits between the barriers
+            // this thread's two rows over the groups
+            float all[2], sum[2], f[KW][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                all[h] = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < KW; ++k) all[h] = fmaxf(all[h], ctl.ml[k * RW + rw][nt * 8 + 2 * t4 + h].x);
+                const float to = all[h] == -INFINITY ? 0.f : all[h];
+                sum[h] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KW; ++k) {
+                    const float2 v = ctl.ml[k * RW + rw][nt * 8 + 2 * t4 + h];
+                    f[k][h] = ex2_approx(v.x - to);
+                    sum[h] += v.y * f[k][h];
+                }
             }
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int row0 = rw * 8 * NT + nt * 8;
+            float out_f[2];
 #pragma unroll
-            for (int k = 0; k < kHalf; ++k) {
-                const float4 v = *reinterpret_cast<const float4*>(slot_at(k * RW + rwi, r16, col));
-                acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+            for (int h = 0; h < 2; ++h) out_f[h] = from_start && to_end ? v_scale / sum[h] : 1.f;
+            // where this thread's words go: row g8 of the row tile
+            const int r = row0 + g8, rr = x.rt * S::kRows + r, tok = rr / p.group, head = x.kvh * p.group + (rr - tok * p.group);
+            T* dst = static_cast<T*>(p.o) + (long long)(x.s.first + tok) * p.o_stride + (long long)head * D;
+#pragma unroll
+            for (int i = 0; i < S::kSlice; ++i) {
+                const int dt = kw * S::kSlice + i;
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KW; ++k) {
+                    float2 a, b;
+                    if (k == kw) {
+#pragma unroll
+                        for (int j = 0; j < KW; ++j)
+                            if (j == kw) {
+                                const float(&w)[4] = o[nt][j * S::kSlice + i];
+                                a = make_float2(w[0], w[1]), b = make_float2(w[2], w[3]);
+                            }
+                    } else {
+                        a = *slot_at(k, kw, i, 0), b = *slot_at(k, kw, i, 1);
+                    }
+                    v[0] += a.x * f[k][0], v[1] += a.y * f[k][1], v[2] += b.x * f[k][0], v[3] += b.y * f[k][1];
+                }
+                if (from_start && to_end) {
+                    // a row without keys is zero; rows out as 16-bit pairs along head_dim
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = all[j & 1] == -INFINITY ? 0.f : v[j] * out_f[j & 1];
+                    const uint32_t a = movmatrix_trans(Half16<T>::pack(v[0], v[1])), b = movmatrix_trans(Half16<T>::pack(v[2], v[3]));
+                    if (r < tile_rows) {
+                        if constexpr (kE4m3) {
+                            *reinterpret_cast<uint2*>(dst + dt * 16 + 4 * t4) = make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+                        } else {
+                            *reinterpret_cast<uint32_t*>(dst + dt * 16 + 2 * t4) = a;
+                            *reinterpret_cast<uint32_t*>(dst + dt * 16 + 8 + 2 * t4) = b;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int row = row0 + 2 * t4 + h;
+                        if (row >= tile_rows) continue;
+                        float* ws = p.ws_o + ((long long)share * S::kRows + row) * D + dt * 16;
+                        if constexpr (kE4m3) {
+                            *reinterpret_cast<float2*>(ws + 2 * g8) = make_float2(v[h], v[2 + h]);
+                        } else {
+                            ws[g8] = v[h];
+                            ws[8 + g8] = v[2 + h];
+                        }
+                    }
+                }
             }
-            if (from_start && to_end) {
-                const int rr = x.rt * S::kRows + r, tok = rr / p.group, head = x.kvh * p.group + (rr - tok * p.group);
-                const long long t = x.s.first + tok;
-                const float f = v_scale / sum;                // a row without keys is zero
-                *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + t * p.o_stride + (long long)head * D + col) =
-                    all == -INFINITY ? make_uint2(0u, 0u) : make_uint2(Half16<T>::pack(acc.x * f, acc.y * f), Half16<T>::pack(acc.z * f, acc.w * f));
-                if (p.lse != nullptr && col == 0)
-                    p.lse[t * p.n_heads + head] = all == -INFINITY ? -INFINITY : (all + log2f(sum)) * 0.69314718055994531f;
-            } else {
-                *reinterpret_cast<float4*>(p.ws_o + ((long long)share * S::kRows + r) * D + col) = acc;
-                if (col == 0) p.ws_ml[share * S::kRows + r] = make_float2(all, sum);
+            if (kw == 0 && g8 == 0) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = row0 + 2 * t4 + h;
+                    if (row >= tile_rows) continue;
+                    if (!(from_start && to_end)) {
+                        p.ws_ml[share * S::kRows + row] = make_float2(all[h], sum[h]);
+                    } else if (p.lse != nullptr) {
+                        const int at_row = x.rt * S::kRows + row, i = at_row / p.group;
+                        p.lse[(long long)(x.s.first + i) * p.n_heads + x.kvh * p.group + (at_row - i * p.group)] =
+                            all[h] == -INFINITY ? -INFINITY : (all[h] + log2f(sum[h])) * 0.69314718055994531f;
+                    }
+                }
             }
         }
         __syncthreads();
-        at = walk.work_end;
+        if (stopped) break;
     }
 
     if (*abort_flag != 0u) {
@@ -521,10 +597,8 @@ paged_join_kernel(const __grid_constant__ AttendParams p, int rows) {
     const int4 job = p.ws_join[cta];
     if (job.w == 0) return;
     const int row = blockIdx.y * 4 + warp, rr = job.z * rows + row, tok = rr / p.group;
-    Where x;
-    x.b = job.x;
-    load_seq(p, rows, 16, x);
-    if (tok >= x.s.n_new) return;
+    const SeqView s = seq_of(p.batch, p.page_shift, job.x);
+    if (tok >= s.n_new) return;
     auto share = [&](int j) { return share_of(cta - 1 + j, j == 0); };
     float all = -INFINITY;
     for (int j = lane; j < job.w; j += 32) all = fmaxf(all, p.ws_ml[share(j) * rows + row].x);
@@ -555,7 +629,7 @@ paged_join_kernel(const __grid_constant__ AttendParams p, int rows) {
         }
     }
     const int head = job.y * p.group + (rr - tok * p.group);
-    const long long t = x.s.first + tok;
+    const long long t = s.first + tok;
     const float f = (kE4m3 && p.v_scale ? p.v_scale[job.y] : 1.f) / sum;
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + t * p.o_stride + (long long)head * D + lane * kCols);
 #pragma unroll
@@ -564,18 +638,29 @@ paged_join_kernel(const __grid_constant__ AttendParams p, int rows) {
         p.lse[t * p.n_heads + head] = all == -INFINITY ? -INFINITY : (all + log2f(sum)) * 0.69314718055994531f;
 }
 
-template <class T, bool kE4m3, int D, int RW>
-cudaError_t prepare_one() {
-    return cudaFuncSetAttribute(paged_token_kernel<T, kE4m3, D, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)Shape<kE4m3, D, RW>::kSmem + 1024);
+// The variant for a tile of `rows` rows: f(NT, RW). 64-wide heads have registers for four row tiles a warp, and then read K and
+// V from shared memory once for 32 rows.
+template <int D, class F>
+cudaError_t with_rows(int rows, F&& f) {
+    using std::integral_constant;
+    constexpr int kWide = D == 64 ? 4 : 2;
+    if (rows == 8) return f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    if (rows == 16) return f(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+    if (rows == 32) return f(integral_constant<int, kWide>{}, integral_constant<int, 4 / kWide>{});
+    return f(integral_constant<int, kWide>{}, integral_constant<int, 8 / kWide>{});
 }
+
 template <class T, bool kE4m3, int D>
-cudaError_t prepare_rows() {
+cudaError_t prepare() {
     cudaFuncAttributes attr;
-    cudaError_t e = prepare_one<T, kE4m3, D, 1>();
-    if (e == cudaSuccess) e = prepare_one<T, kE4m3, D, 2>();
-    if (e == cudaSuccess) e = prepare_one<T, kE4m3, D, 4>();
-    if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, paged_join_kernel<T, kE4m3, D>);
+    cudaError_t e = cudaFuncGetAttributes(&attr, paged_join_kernel<T, kE4m3, D>);
+    for (int rows : {8, 16, 32, 64})
+        if (e == cudaSuccess)
+            e = with_rows<D>(rows, [](auto nt, auto rw) {
+                constexpr int NT = decltype(nt)::value, RW = decltype(rw)::value;
+                return cudaFuncSetAttribute(paged_token_kernel<T, kE4m3, D, NT, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            (int)Shape<kE4m3, D, NT, RW>::kSmem + 1024);
+            });
     return e;
 }
 
@@ -587,12 +672,14 @@ cudaError_t launch(const AttendParams& p, int rows, int used_rows, cudaStream_t 
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.n_ctas);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Shape<kE4m3, D, 1>::kSmem + 1024;   // the same for 16, 32 and 64 rows
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, rows == 16 ? paged_token_kernel<T, kE4m3, D, 1>
-                                             : rows == 32 ? paged_token_kernel<T, kE4m3, D, 2> : paged_token_kernel<T, kE4m3, D, 4>, p);
+    const cudaError_t e = with_rows<D>(rows, [&](auto nt, auto rw) {
+        constexpr int NT = decltype(nt)::value, RW = decltype(rw)::value;
+        cfg.dynamicSmemBytes = Shape<kE4m3, D, NT, RW>::kSmem + 1024;
+        return cudaLaunchKernelEx(&cfg, paged_token_kernel<T, kE4m3, D, NT, RW>, p);
+    });
     if (e != cudaSuccess || p.n_ctas == 1) return e;
     cfg.gridDim = dim3(p.n_ctas, (used_rows + 3) / 4);
     cfg.blockDim = dim3(128);
@@ -612,10 +699,11 @@ cudaError_t with_types(PagedType type, PagedType cache, int head_dim, F&& f) {
 
 }  // namespace
 
-int token_rows(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+int token_rows(long long rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+int token_ctas(int sms) { return kCtasPerSm * sms; }
 
 cudaError_t paged_token_prepare(PagedType type, PagedType cache, int head_dim) {
-    return with_types(type, cache, head_dim, [](auto t, auto e, auto d) { return prepare_rows<decltype(t), decltype(e)::value, decltype(d)::value>(); });
+    return with_types(type, cache, head_dim, [](auto t, auto e, auto d) { return prepare<decltype(t), decltype(e)::value, decltype(d)::value>(); });
 }
 
 cudaError_t paged_token_launch(const AttendParams& p, PagedType type, PagedType cache, int head_dim, int rows, int used_rows,

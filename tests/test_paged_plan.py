@@ -44,17 +44,16 @@ static void one(std::mt19937& r, bool wild) {
     p.batch = PagedBatch{cu.data(), lens.data(), nullptr, width, width, n, n_tokens};
     const int n_ctas = pick(1, 12);
 
+    auto seq = [&](int b) { return seq_of(p.batch, p.page_shift, b); };
     unsigned total = 0;
     std::vector<unsigned> start;
     for (int b = 0; b < n; ++b) {
-        Where x; x.b = b;
-        load_seq(p, kRows, kUnit, x);
         start.push_back(total);
-        total += seq_units(p, x.w);
+        total += seq_places(p, seq_work(seq(b), p.group, kRows, kUnit, p.window));
     }
     start.push_back(total);
     if (total == 0) return;
-    const int n_pieces = pieces(total, n_ctas, KW);
+    const int n_pieces = pieces(total, n_ctas, kWorkCost + KW);
     CHECK(piece_begin(total, n_pieces, 0) == 0 && piece_begin(total, n_pieces, n_pieces) == total);
     using Id = std::tuple<int, int, int>;                       // sequence, head, row tile
     std::map<Id, std::set<int>> keys;                           // units taken
@@ -64,47 +63,46 @@ static void one(std::mt19937& r, bool wild) {
     std::map<Id, int> whole;
     for (int c = 0; c < n_pieces; ++c) {
         const unsigned begin = piece_begin(total, n_pieces, c), end = piece_begin(total, n_pieces, c + 1);
-        CHECK(end > begin && (n_pieces == 1 || end - begin >= KW));
+        CHECK(end > begin);
         int b0 = 0;
         while (start[b0 + 1] <= begin) ++b0;
         Where first; first.b = b0; first.seq_begin = start[b0];
-        load_seq(p, kRows, kUnit, first);
+        first.s = seq(b0);
+        first.w = seq_work(first.s, p.group, kRows, kUnit, p.window);
         for (int kw = 0; kw < KW; ++kw) {
             // the fetching warp's walk and the consuming one's have to be the same
             std::vector<std::pair<Id, int>> fetched, used;
             Units<kRows, kUnit, KW> a;
             a.x = first; a.end = end; a.kw = kw;
-            for (a.enter(p, begin); a.more; a.next(p)) {
+            for (a.enter(p, seq, begin); a.more; a.next(p, seq)) {
                 CHECK(a.x.b < n && a.x.kvh < p.n_kv_heads && a.x.rt < a.x.w.row_tiles);
                 CHECK(a.key0() >= 0 && a.key0() < a.x.hi && a.x.hi <= capacity);
                 fetched.push_back({Id{a.x.b, a.x.kvh, a.x.rt}, a.key0()});
             }
             Units<kRows, kUnit, KW> w;
             w.x = first; w.end = end; w.kw = kw;
-            for (unsigned at = begin; at < end;) {
-                find_work(p, kRows, kUnit, at, w.x);
-                const unsigned work_end = w.x.work_begin + (unsigned)w.x.w.n_units;
-                w.work_end = least_of(end, work_end);
-                w.u = at + kw;
+            for (unsigned at = begin; at < end; at = w.stop) {
+                const bool any = w.begin(p, seq, at);
+                if (kw == 0 && at == begin) {
+                    const int m = shares_to_join(w.x, total, n_pieces, c);
+                    if (m) {
+                        const Id id{w.x.b, w.x.kvh, w.x.rt};
+                        CHECK(joined.count(id) == 0 && m >= 2);
+                        for (int j = 0; j < m; ++j) joined[id].push_back(share_of(c - 1 + j, j == 0));
+                    }
+                }
+                if (!any) { CHECK(w.stop == end); break; }
                 const Id id{w.x.b, w.x.kvh, w.x.rt};
                 for (bool have = w.settle(); have; w.u += KW, have = w.settle()) used.push_back({id, w.key0()});
                 if (kw == 0) {
-                    const bool from_start = at == w.x.work_begin, to_end = w.work_end == work_end;
+                    const bool from_start = at <= w.x.first_unit(), to_end = w.stop == w.x.work_end;
                     if (from_start && to_end) ++whole[id];
                     else {
                         const int s = share_of(c, from_start);
                         CHECK(s >= 0 && s < 2 * n_ctas && share_used.insert(s).second);
                         shares[id].push_back(s);
                     }
-                    if (at == begin) {
-                        const int m = shares_to_join(w.x, total, n_pieces, c);
-                        if (m) {
-                            CHECK(joined.count(id) == 0 && m >= 2);
-                            for (int j = 0; j < m; ++j) joined[id].push_back(share_of(c - 1 + j, j == 0));
-                        }
-                    }
                 }
-                at = w.work_end;
             }
             CHECK(fetched == used);
             for (auto& [id, k] : used) CHECK(keys[id].insert(k).second);
@@ -112,8 +110,9 @@ static void one(std::mt19937& r, bool wild) {
     }
     CHECK(shares == joined);
     for (int b = 0; b < n; ++b) {
-        Where x; x.b = b;
-        load_seq(p, kRows, kUnit, x);
+        Where x;
+        x.s = seq(b);
+        x.w = seq_work(x.s, p.group, kRows, kUnit, p.window);
         CHECK(x.s.first >= 0 && x.s.n_new >= 0 && x.s.first + x.s.n_new <= n_tokens && x.s.len >= 0 && x.s.len <= capacity);
         for (int h = 0; h < p.n_kv_heads; ++h)
             for (int rt = 0; rt < x.w.row_tiles; ++rt) {
@@ -134,10 +133,10 @@ int main() {
     for (case_no = 0; case_no < 800; ++case_no) {
         const bool wild = case_no % 3 == 2;
         switch (case_no % 4) {
-            case 0: one<16, 16, 8>(r, wild); break;
-            case 1: one<16, 32, 8>(r, wild); break;
-            case 2: one<32, 32, 4>(r, wild); break;
-            default: one<64, 16, 2>(r, wild);
+            case 0: one<8, 16, 4>(r, wild); break;
+            case 1: one<16, 32, 4>(r, wild); break;
+            case 2: one<32, 16, 2>(r, wild); break;
+            default: one<64, 16, 1>(r, wild);
         }
     }
     return 0;
