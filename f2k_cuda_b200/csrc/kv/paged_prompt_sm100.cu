@@ -125,12 +125,18 @@ __device__ __forceinline__ bool find_job(const AttendParams& p, int tokens_per_t
     return false;
 }
 
+// Shared memory of a tile's Q, and later of its rows on their way out: there 16 bytes apart, against bank conflicts.
+template <int D>
+constexpr uint32_t kQArea = kRows * (D * 2 + 16);
+template <int D>
+constexpr int kSmemBytes = 2 * (int)kQArea<D> + kStages * (D / 64) * (int)kPieceBytes + 1024;
+
 template <class T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     constexpr int kPieces = D / 64;                     // 128-byte pieces of a row
     constexpr uint32_t kTileBytes = kPieces * kPieceBytes;
-    constexpr uint32_t kSmemQ = 0, kSmemRing = 2 * kTileBytes;
+    constexpr uint32_t kQBytes = kQArea<D>, kSmemQ = 0, kSmemRing = 2 * kQBytes;
     constexpr uint32_t kFormat = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Ctl ctl_;
@@ -250,7 +256,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             // ------------------------------ MMA issuer, converged ------------------------------
             constexpr uint32_t idesc_s = umma_idesc_16(kRows, kKeys, false, kFormat), idesc_o = umma_idesc_16(kRows, D, true, kFormat);
             bool ok = true;
-            const uint64_t q0_desc = umma_smem_desc(smem + kSmemQ, 16, 1024), q1_desc = umma_smem_desc(smem + kSmemQ + kTileBytes, 16, 1024);
+            const uint64_t q0_desc = umma_smem_desc(smem + kSmemQ, 16, 1024), q1_desc = umma_smem_desc(smem + kSmemQ + kQBytes, 16, 1024);
             const uint64_t k_desc0 = umma_smem_desc(smem + kSmemRing, 16, 1024), v_desc0 = umma_smem_desc(smem + kSmemRing, kPieceBytes, 1024);
             const uint32_t bar_full0 = smem_u32(&ctl->kv_full[0]), bar_empty0 = smem_u32(&ctl->kv_empty[0]), bar_free = smem_u32(&ctl->s_free);
             // Ring slot of K_j is 2j, of V_j is 2j+1. Every wait is looked at ahead, in front of the MMAs before it.
@@ -340,24 +346,33 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         const float c = p.scale_log2;
         const int tok0 = (job.tile0 + t) * per_tile, rows = min(per_tile, job.s.n_new - tok0) * p.group;
         constexpr int kChunks = D / 8;                  // 16-byte chunks of a row
-        const uint32_t q_tile = smem + kSmemQ + t * kTileBytes;
-        {   // Q rows to shared memory as the MMA reads them: 128-byte pieces, chunks swizzled by row
-            const int tid = threadIdx.x & 127;
-            const T* q = static_cast<const T*>(p.q) + (long long)(job.s.first + tok0) * p.q_stride + (long long)kvh * p.group * D;
-#pragma unroll 4
-            for (int i = tid; i < kRows * kChunks; i += 128) {
-                const int r = i / kChunks, ch = i % kChunks, tok = r / p.group;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < rows) v = *reinterpret_cast<const uint4*>(q + tok * p.q_stride + (r - tok * p.group) * D + ch * 8);
-                st_shared_v4(q_tile + (ch >> 3) * kPieceBytes + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v);
+        const uint32_t q_tile = smem + kSmemQ + t * kQBytes;
+        // Row r of a tile is token r / group: by a multiplication (r < 128, group <= 128), a division per row cost more than the row.
+        const uint32_t over_group = (65536u + (uint32_t)p.group - 1u) / (uint32_t)p.group;
+        auto token_of = [&](int r) { return (int)((uint32_t)r * over_group >> 16); };
+        constexpr int kAtOnce = 32 / kChunks;           // rows that a warp reads or writes at once
+        const int ch = lane % kChunks, first_row = (warp & 3) * 32 + lane / kChunks;
+        {   // Q rows to shared memory as the MMA reads them: 128-byte pieces, chunks swizzled by row. All loads first.
+            const T* q = static_cast<const T*>(p.q) + (long long)(job.s.first + tok0) * p.q_stride + (long long)kvh * p.group * D + ch * 8;
+            uint4 v[kChunks];
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+                const int r = first_row + i * kAtOnce, tok = token_of(r);
+                v[i] = make_uint4(0, 0, 0, 0);
+                if (r < rows) v[i] = *reinterpret_cast<const uint4*>(q + tok * p.q_stride + (r - tok * p.group) * D);
+            }
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+                const int r = first_row + i * kAtOnce;
+                st_shared_v4(q_tile + (ch >> 3) * kPieceBytes + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v[i]);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&ctl->q_full[t]));
         }
         const int r = (warp & 3) * 32 + lane;
-        KeyRange see{0, 0};                             // of this thread's row
-        if (r < rows) see = visible_keys(job.s, tok0 + r / p.group, p.window);
+        KeyRange see{0, 0x7fffffff};                    // of this thread's row; rows that do not exist are not masked
+        if (r < rows) see = visible_keys(job.s, tok0 + token_of(r), p.window);
         float m_ref = -INFINITY, l_sum = 0.0f;
         bool ok = true;
         const uint32_t all_boxes = (1u << (kKeys / min(kKeys, 1 << p.page_shift))) - 1u;
@@ -368,10 +383,10 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             if (!ok) break;
             tc_fence_after_sync();
             const int base = key00 + j * kKeys;
-            const uint32_t boxes = *reinterpret_cast<volatile uint32_t*>(&ctl->boxes[j % kBoxRing]);
-            const bool masked = __any_sync(0xffffffffu, base < see.lo || base + kKeys > see.hi) || boxes != all_boxes;
             uint32_t s[128];
             float mx[kMaxChains];
+            uint32_t boxes;
+            bool masked;
             auto hide = [&](int from) {                 // scores [from, from + 64) of keys that the row does not see
                 const int first = see.lo - base, end = see.hi - base;
 #pragma unroll
@@ -393,6 +408,8 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 uint32_t(&s3)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[96]);
                 tmem_ld_x32(tS + 0, s0);
                 tmem_ld_x32(tS + 32, s1);
+                boxes = *reinterpret_cast<volatile uint32_t*>(&ctl->boxes[j % kBoxRing]);
+                masked = __any_sync(0xffffffffu, base < see.lo || base + kKeys > see.hi) || boxes != all_boxes;
                 tmem_wait_ld();
                 tmem_ld_x32(tS + 64, s2);
                 tmem_ld_x32(tS + 96, s3);
@@ -472,8 +489,9 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             tc_fence_after_sync();
             const bool none = l_sum == 0.0f && m_ref == -INFINITY;      // a row that sees no key is zero
             const float inv = 1.0f / l_sum;
-            // Rows go out through the shared memory of the tile's Q (no MMA reads it any more), chunk c of row r at
-            // position c ^ (r mod chunks), so that a row leaves in whole lines.
+            // Rows go out through the shared memory of the tile's Q (no MMA reads it any more), a bulk copy each: 16-byte stores by
+            // half-warps kept the CTA 6000 to 7000 clk.
+            const uint32_t park = q_tile + r * (D * 2 + 16);
 #pragma unroll
             for (int q = 0; q < D / 32; ++q) {
                 uint32_t o[32];
@@ -489,26 +507,17 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                     v.z = Half16<T>::pack(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
                     v.w = Half16<T>::pack(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
                     if (none) v = make_uint4(0, 0, 0, 0);
-                    const int ch = q * 4 + (i >> 3);
-                    st_shared_v4(q_tile + r * (D * 2) + ((ch ^ (r & (kChunks - 1))) << 4), v);
+                    st_shared_v4(park + (q * 4 + (i >> 3)) * 16, v);
                 }
             }
-            if (p.lse != nullptr && r < rows) {
-                const int tok = r / p.group;
-                p.lse[(long long)(job.s.first + tok0 + tok) * p.n_heads + kvh * p.group + (r - tok * p.group)] =
-                    none ? -INFINITY : (m_ref * c + log2f(l_sum)) * 0.69314718055994531f;
-            }
-            __syncwarp();
-            constexpr int kRowsAtOnce = 32 / kChunks;
-            const int ch = lane % kChunks;
-            T* out = static_cast<T*>(p.o) + (long long)(job.s.first + tok0) * p.o_stride + (long long)kvh * p.group * D + ch * 8;
-#pragma unroll 4
-            for (int i = lane / kChunks; i < 32; i += kRowsAtOnce) {
-                const int row = (warp & 3) * 32 + i;
-                if (row >= rows) break;
-                const int tok = row / p.group;
-                *reinterpret_cast<uint4*>(out + tok * p.o_stride + (row - tok * p.group) * D) =
-                    ld_shared_v4(q_tile + row * (D * 2) + ((ch ^ (row & (kChunks - 1))) << 4));
+            fence_proxy_async_smem();
+            if (r < rows) {
+                const int tok = token_of(r), head = kvh * p.group + (r - tok * p.group);
+                const long long at = job.s.first + tok0 + tok;
+                bulk_store(static_cast<T*>(p.o) + at * p.o_stride + (long long)head * D, park, D * 2);
+                bulk_commit();
+                if (p.lse != nullptr) p.lse[at * p.n_heads + head] = none ? -INFINITY : (m_ref * c + log2f(l_sum)) * 0.69314718055994531f;
+                bulk_wait_read<0>();
             }
         }
     }
@@ -523,9 +532,6 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     }
 }
 
-template <int D>
-constexpr int smem_bytes() { return (2 + kStages) * (D / 64) * (int)kPieceBytes + 1024; }
-
 template <class F>
 cudaError_t with_types(PagedType type, int head_dim, F&& f) {
     auto by_dim = [&](auto t) { return head_dim == 64 ? f(t, std::integral_constant<int, 64>{}) : f(t, std::integral_constant<int, 128>{}); };
@@ -537,7 +543,7 @@ cudaError_t with_types(PagedType type, int head_dim, F&& f) {
 cudaError_t paged_prompt_prepare(PagedType type, int head_dim) {
     return with_types(type, head_dim, [](auto t, auto d) {
         return cudaFuncSetAttribute(paged_prompt_kernel<decltype(t), decltype(d)::value>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    smem_bytes<decltype(d)::value>());
+                                    kSmemBytes<decltype(d)::value>);
     });
 }
 
@@ -557,7 +563,7 @@ cudaError_t paged_prompt_launch(const AttendParams& p, PagedType type, int head_
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)ctas(per_cta));
         cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = smem_bytes<decltype(d)::value>();
+        cfg.dynamicSmemBytes = kSmemBytes<decltype(d)::value>;
         cfg.stream = stream;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
