@@ -2,18 +2,24 @@
 //
 // A tile is 128 query rows of one sequence and key head: 128 / group new tokens with the `group` query heads of the key
 // head side by side (fewer rows where group does not divide 128), so a key and its value are read once for all heads
-// that share them, and the rows of a tile see nearly the same keys. A CTA has two neighbouring tiles, or one, and walks
-// the 128-key tiles between the first key that its first token sees and the last that its last one sees.
+// that share them, and the rows of a tile see nearly the same keys. A CTA walks the 128-key tiles between the first key
+// that its first token sees and the last that its last one sees, in one of two forms:
 //
-// Roles as in the joint-attention kernel (attn_fwd_sm100.cu): warps 0-3 / 4-7 the softmax of tile 0 / 1 (one thread per
-// row), warp 8 the loader, warp 9 the tcgen05 issuer, one S buffer in tensor memory that the tiles use in turn, P from
-// tensor memory, lazily moved reference maxima. What differs:
+//   pair    two neighbouring query tiles, every key tile meets both: half the reads of the other form;
+//   split   one query tile, its even key tiles for one softmax group and its odd ones for the other, joined at the end
+//           through shared memory: CTAs half as long, for batches that do not fill the GPU with pairs, and for the odd last
+//           tile of a sequence. (One group on all key tiles leaves the special-function unit and the tensor pipe idle
+//           half the time: 1024 tokens behind 15001, 16 heads of 64, 154 us.)
 //
-//  * The loader brings a key tile in page by page: a lane per page and 128-byte piece of head_dim looks its page up (a
+// Roles as in the joint-attention kernel (attn_fwd_sm100.cu): warps 0-3 / 4-7 the softmax groups (one thread per row),
+// warps 8 and 10 the loaders of K and V, warp 9 the tcgen05 issuer, one S buffer in tensor memory that the groups use in turn, P
+// from tensor memory, lazily moved reference maxima. What differs:
+//
+//  * A loader brings a key tile in page by page: a lane per page and 128-byte piece of head_dim looks its page up (a
 //    tile ahead) and issues its own TMA box. Rows of V that no query of the CTA may see - the rest of the last page,
 //    pages in front of a window, pages outside the cache - hold anything, and 0 * NaN is NaN in a product, so the loader
 //    waits for such a tile and clears them before it hands the tile over. That is the last tile, or the first ones of a
-//    window.
+//    window. K and V have a ring and a loader each: K of the tile after next may come in as soon as S is done with its slot.
 //  * Q is fetched by the softmax groups themselves (the rows of a tile are a gather once group is not a power of two).
 //  * Scores are masked by key number, only in tiles that some row of the warp does not see whole.
 //
@@ -34,23 +40,27 @@ using namespace f2k::ptx;
 
 namespace {
 
-constexpr int kThreads = 384, kLoaderWarp = 8, kMmaWarp = 9;
-constexpr int kStages = 4;
+constexpr int kThreads = 384, kLoadK = 8, kMmaWarp = 9, kLoadV = 10;
 constexpr int kRows = 128, kKeys = kPromptTile;
 constexpr uint32_t kPieceBytes = 128 * 128;             // 128 rows of 128 bytes
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColP0 = 128, kColP1 = 192, kColO0 = 256, kColO1 = 384;
 constexpr float kLazyThreshold = 8.0f;                  // log2 units
 constexpr int kPParts = 2;
-constexpr int kBoxRing = 8;                             // tiles whose page flags are kept; the loader is at most three ahead
+constexpr int kBoxRing = 16;                            // tiles whose page flags are kept; the loader is at most six ahead
+
+constexpr int kMostStages = 4;
+template <int D>
+constexpr int kStages = D == 64 ? 4 : 2;                // tiles of K, and of V, in flight or in use: 64 KB each
 
 struct Ctl {
     uint64_t q_full[2];
-    uint64_t kv_full[kStages];
-    uint64_t kv_empty[kStages];
-    uint64_t s_full[2];
     uint64_t s_free;
     uint64_t p_full[2][kPParts];
+    uint64_t joined;                                    // split form: group 1 has left its share (these: four arrivals each)
+    uint64_t full[2][kMostStages];                      // [K, V][slot]
+    uint64_t empty[2][kMostStages];
+    uint64_t s_full[2];
     uint64_t pv_done[2];
     uint64_t drain;
     uint64_t clean;                                     // a V tile that has to be cleared in part has arrived
@@ -129,14 +139,15 @@ __device__ __forceinline__ bool find_job(const AttendParams& p, int tokens_per_t
 template <int D>
 constexpr uint32_t kQArea = kRows * (D * 2 + 16);
 template <int D>
-constexpr int kSmemBytes = 2 * (int)kQArea<D> + kStages * (D / 64) * (int)kPieceBytes + 1024;
+constexpr int kSmemBytes = 2 * (int)kQArea<D> + 2 * kStages<D> * (D / 64) * (int)kPieceBytes + 1024;
 
 template <class T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     constexpr int kPieces = D / 64;                     // 128-byte pieces of a row
     constexpr uint32_t kTileBytes = kPieces * kPieceBytes;
-    constexpr uint32_t kQBytes = kQArea<D>, kSmemQ = 0, kSmemRing = 2 * kQBytes;
+    constexpr int kSlots = kStages<D>;
+    constexpr uint32_t kQBytes = kQArea<D>, kSmemQ = 0, kSmemRing = 2 * kQBytes;      // K slots, then V slots
     constexpr uint32_t kFormat = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Ctl ctl_;
@@ -149,12 +160,10 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     const long long wait_limit = p.wait_limit_clk;
 
     grid_launch_dependents();
-    if (warp == kLoaderWarp) {
-        constexpr int kBars = offsetof(Ctl, tmem_base) / sizeof(uint64_t);
-        constexpr int kFree = offsetof(Ctl, s_free) / sizeof(uint64_t), kP = offsetof(Ctl, p_full) / sizeof(uint64_t);
+    if (warp == kLoadK) {
+        constexpr int kBars = offsetof(Ctl, tmem_base) / sizeof(uint64_t), kPerWarp = offsetof(Ctl, full) / sizeof(uint64_t);
         static_assert(kBars <= 32, "a lane per barrier");
-        const bool per_warp = lane < 2 || lane == kFree || (lane >= kP && lane < kP + 2 * kPParts);   // a group's four warps arrive
-        if (lane < kBars) mbar_init(smem_u32(ctl) + lane * 8, per_warp ? 4 : 1);
+        if (lane < kBars) mbar_init(smem_u32(ctl) + lane * 8, lane < kPerWarp ? 4 : 1);    // a group's four warps arrive, or one thread
         if (lane == 0) ctl->abort = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
@@ -169,14 +178,17 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     Job job;
     const bool any = find_job(p, per_tile, per_cta, blockIdx.x / p.n_kv_heads, lane, job);
     // Keys that some row of the CTA sees, and the key tiles they lie in.
-    const bool has_t1 = any && job.two;
+    const bool pair = any && job.two;
     int lo = 0, hi = 0;
     if (any) {
         lo = visible_keys(job.s, job.tile0 * per_tile, p.window).lo;
-        hi = visible_keys(job.s, min(job.s.n_new, (job.tile0 + (has_t1 ? 2 : 1)) * per_tile) - 1, p.window).hi;
+        hi = visible_keys(job.s, min(job.s.n_new, (job.tile0 + (pair ? 2 : 1)) * per_tile) - 1, p.window).hi;
     }
     const int key00 = lo / kKeys * kKeys;
     const int n_kv = hi > key00 ? (hi - key00 + kKeys - 1) / kKeys : 0;
+    // Step i of group t is key tile `tile_of(t, i)`, i < steps(t).
+    auto steps = [&](int t) { return pair ? n_kv : (n_kv + 1 - t) >> 1; };
+    auto tile_of = [&](int t, int i) { return pair ? i : 2 * i + t; };
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -185,41 +197,36 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
 
     if (warp >= 8) {
         setmaxnreg_dec<88>();
-        if (warp == kLoaderWarp) {
-            // ------------------------------ loader: a lane per page and piece ------------------------------
+        if (warp == kLoadK || warp == kLoadV) {
+            // ------------------------------ loaders: a lane per page and piece ------------------------------
+            const int kv = warp == kLoadK ? 0 : 1;
             const int box_rows = min(kKeys, 1 << p.page_shift), n_boxes = kKeys / box_rows;
             const int box = lane & 7, piece = lane >> 3;
             const bool mine = box < n_boxes && piece < kPieces;
             const uint32_t all_boxes = (1u << n_boxes) - 1u;
             const int32_t* row = p.batch.table + (any ? job.b : 0) * p.batch.table_stride;
+            const CUtensorMap* map = kv == 0 ? &p.tm_k : &p.tm_v;
             auto needed = [&](int j) {
                 const int k = key00 + j * kKeys + box * box_rows;
                 return mine && j < n_kv && k < hi && k + box_rows > lo;
             };
             auto look_up = [&](int j) { return needed(j) ? row[(key00 + j * kKeys + box * box_rows) >> p.page_shift] : 0; };
-            int page = 0, next_page = look_up(0);
-            bool ok = true, good = false;
-            uint32_t boxes = 0;
-            int issued = 0, cleaned = 0;
-            for (; issued < 2 * n_kv && ok; ++issued) {
-                const int j = issued >> 1, kv = issued & 1, slot = issued % kStages;
-                const int base = key00 + j * kKeys;
-                if (kv == 0) {
-                    page = next_page;
-                    next_page = look_up(j + 1);
-                    const bool wanted = needed(j);
-                    good = wanted && (unsigned)page < (unsigned)p.n_pages;
-                    if (wanted && !good) atomicOr(p.status, (int)kStatusBadPage);
-                    boxes = __ballot_sync(0xffffffffu, good) & 0xFFu;
-                }
-                if (issued >= kStages) {
-                    ok = mbar_wait(smem_u32(&ctl->kv_empty[slot]), ((issued / kStages) & 1) ^ 1u, abort_flag, wait_limit);
+            int next_page = look_up(0), cleaned = 0, j = 0;
+            bool ok = true;
+            for (; j < n_kv; ++j) {
+                const int slot = j % kSlots, base = key00 + j * kKeys, page = next_page;
+                next_page = look_up(j + 1);
+                const bool wanted = needed(j), good = wanted && (unsigned)page < (unsigned)p.n_pages;
+                if (wanted && !good) atomicOr(p.status, (int)kStatusBadPage);
+                const uint32_t boxes = __ballot_sync(0xffffffffu, good) & 0xFFu;
+                if (j >= kSlots) {
+                    ok = mbar_wait(smem_u32(&ctl->empty[kv][slot]), ((j / kSlots) & 1) ^ 1u, abort_flag, wait_limit);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 }
                 const bool clear = kv == 1 && (base < lo || base + kKeys > hi || boxes != all_boxes);
-                const uint32_t full = smem_u32(&ctl->kv_full[slot]), bar = clear ? smem_u32(&ctl->clean) : full;
-                const uint32_t dst = smem + kSmemRing + slot * kTileBytes;
+                const uint32_t full = smem_u32(&ctl->full[kv][slot]), bar = clear ? smem_u32(&ctl->clean) : full;
+                const uint32_t dst = smem + kSmemRing + (kv * kSlots + slot) * kTileBytes;
                 if (lane == 0) {
                     if (kv == 0) ctl->boxes[j % kBoxRing] = boxes;
                     mbar_arrive_expect_tx(bar, (uint32_t)__popc(boxes) * kPieces * (uint32_t)box_rows * 128u);
@@ -227,7 +234,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 __syncwarp();
                 if (good) {
                     const int first = (base + box * box_rows) & ((1 << p.page_shift) - 1);
-                    tma_load_5d(dst + piece * kPieceBytes + box * box_rows * 128, kv == 0 ? &p.tm_k : &p.tm_v, bar, 0, first, piece, kvh, page);
+                    tma_load_5d(dst + piece * kPieceBytes + box * box_rows * 128, map, bar, 0, first, piece, kvh, page);
                 }
                 if (clear) {
                     ok = mbar_wait(bar, cleaned & 1, abort_flag, wait_limit);
@@ -248,86 +255,105 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             if (!ok) {
                 // Leaving early: let the copies this warp started land first (bounded).
                 volatile uint32_t never = 0;
-                mbar_wait(smem_u32(&ctl->clean), cleaned & 1, &never, 4000000ll);
-                for (int i = max(0, issued - kStages); i < issued; ++i)
-                    mbar_wait(smem_u32(&ctl->kv_full[i % kStages]), (i / kStages) & 1, &never, 40000000ll);
+                if (kv == 1) mbar_wait(smem_u32(&ctl->clean), cleaned & 1, &never, 4000000ll);
+                for (int i = max(0, j - kSlots); i < j; ++i)
+                    mbar_wait(smem_u32(&ctl->full[kv][i % kSlots]), (i / kSlots) & 1, &never, 40000000ll);
             }
         } else if (warp == kMmaWarp) {
             // ------------------------------ MMA issuer, converged ------------------------------
             constexpr uint32_t idesc_s = umma_idesc_16(kRows, kKeys, false, kFormat), idesc_o = umma_idesc_16(kRows, D, true, kFormat);
             bool ok = true;
-            const uint64_t q0_desc = umma_smem_desc(smem + kSmemQ, 16, 1024), q1_desc = umma_smem_desc(smem + kSmemQ + kQBytes, 16, 1024);
-            const uint64_t k_desc0 = umma_smem_desc(smem + kSmemRing, 16, 1024), v_desc0 = umma_smem_desc(smem + kSmemRing, kPieceBytes, 1024);
-            const uint32_t bar_full0 = smem_u32(&ctl->kv_full[0]), bar_empty0 = smem_u32(&ctl->kv_empty[0]), bar_free = smem_u32(&ctl->s_free);
-            // Ring slot of K_j is 2j, of V_j is 2j+1. Every wait is looked at ahead, in front of the MMAs before it.
-            auto slot_off16 = [&](int n) { return (uint32_t)(n % kStages) * (kTileBytes >> 4); };
+            const uint64_t q0_desc = umma_smem_desc(smem + kSmemQ, 16, 1024), q1_desc = umma_smem_desc(smem + kSmemQ + (pair ? kQBytes : 0), 16, 1024);
+            const uint64_t k_desc0 = umma_smem_desc(smem + kSmemRing, 16, 1024);
+            const uint64_t v_desc0 = umma_smem_desc(smem + kSmemRing + kSlots * kTileBytes, kPieceBytes, 1024);
+            const uint32_t bar_full0 = smem_u32(&ctl->full[0][0]), bar_empty0 = smem_u32(&ctl->empty[0][0]), bar_free = smem_u32(&ctl->s_free);
+            // Every wait is looked at ahead, in front of the MMAs before it; a look at a barrier that the warp has seen complete
+            // before (the second group's at a tile of a pair) costs nothing more.
+            auto slot_off16 = [&](int j) { return (uint32_t)(j % kSlots) * (kTileBytes >> 4); };
             const WarpBarriers bars{abort_flag, wait_limit};
             auto peek = [&](auto... bar_and_parity) { return look_at(bars, bar_and_parity...); };
             auto finish = [&](const Look& l) { return f2k::finish(bars, l); };
-            auto bar_full = [&](int n) { return bar_full0 + (n % kStages) * 8; };
-            auto par_full = [&](int n) { return (uint32_t)(n / kStages) & 1u; };
-            auto release = [&](int n) { umma_commit(bar_empty0 + (n % kStages) * 8); };
+            auto bar_full = [&](int kv, int j) { return bar_full0 + (kv * kMostStages + j % kSlots) * 8; };
+            auto par_full = [&](int j) { return (uint32_t)(j / kSlots) & 1u; };
+            auto release = [&](int kv, int j) { umma_commit(bar_empty0 + (kv * kMostStages + j % kSlots) * 8); };
             auto bar_p = [&](int t, int part) { return smem_u32(&ctl->p_full[t][part]); };
-            auto issue_s = [&](int t, int j) {
-                tc_fence_after_sync();
-                const uint64_t q = t == 0 ? q0_desc : q1_desc, k = k_desc0 + slot_off16(2 * j);
-                if constexpr (kPieces == 2) umma_ss_x8(tmem + kColS, q, k, idesc_s);
-                else umma_ss_x4(tmem + kColS, q, k, idesc_s);
-                umma_commit(smem_u32(&ctl->s_full[t]));
-            };
-            // O_t (+)= P_t V_j, half by half as the softmax group hands P over; `next` takes the look at what follows.
-            auto issue_pv = [&](int t, int j, const Look& first, auto&& next) -> bool {
-                const uint32_t d = tmem + (t == 0 ? kColO0 : kColO1), a = tmem + (t == 0 ? kColP0 : kColP1);
-                const uint64_t v = v_desc0 + slot_off16(2 * j + 1);
-                if (!finish(first)) return false;
-                const Look half = peek(bar_p(t, 1), (uint32_t)j & 1u);
-                tc_fence_after_sync();
-                umma_ts_x4(d, a, v, idesc_o, j > 0 ? 1u : 0u);
-                if (!finish(half)) return false;
-                next();
-                tc_fence_after_sync();
-                umma_ts_x4(d, a + 32, v + 4 * (2048 >> 4), idesc_o, 1u);
-                umma_commit(smem_u32(&ctl->pv_done[t]));
-                return true;
-            };
-            // With two tiles S0_j is use 2j of the S buffer and S1_j use 2j + 1, with one S0_j is use j; use u waits for
-            // release u - 1.
-            Look look_s{}, look_p{};
-            if (n_kv > 0) {
-                ok = bars.wait(bar_full(0), par_full(0)) && bars.wait(smem_u32(&ctl->q_full[0]), 0);
-                if (ok) issue_s(0, 0);
-                if (ok && has_t1) ok = bars.wait(smem_u32(&ctl->q_full[1]), 0);
-                look_s = peek(bar_free, 0u);
-            }
-            for (int j = 0; j < n_kv && ok; ++j) {
-                if (has_t1) {
-                    if (!(ok = finish(look_s))) break;
-                    if (j > 0) look_p = peek(bar_p(1, 0), (uint32_t)(j - 1) & 1u);
-                    issue_s(1, j);
-                }
-                release(2 * j);
-                auto look_next_s0 = [&] {
-                    if (j + 1 < n_kv)
-                        look_s = peek(bar_full(2 * j + 2), par_full(2 * j + 2), bar_free, has_t1 ? 1u : (uint32_t)(j & 1));
+            // The order is S0_0, then S1_i, P1 V_(i-1), S0_(i+1), P0 V_i: S0_i is use 2i of the S buffer and S1_i use 2i + 1, and a use
+            // waits for the release of the one before. The two forms are compiled apart: this warp's instructions are what a tile
+            // costs (with `pair` looked at as it goes the pair form took 6 % longer).
+            auto run = [&](auto form) {
+                constexpr bool kPair = decltype(form)::value;
+                auto tile = [](int t, int i) { return kPair ? i : 2 * i + t; };
+                const int n0 = kPair ? n_kv : (n_kv + 1) >> 1, n1 = kPair ? n_kv : n_kv >> 1;
+                auto look_s = [&](int t, int i) {
+                    const int j = tile(t, i);
+                    if (kPair && t == 1) return peek(bar_free, 0u);                    // K_i is there
+                    return peek(bar_full(0, j), par_full(j), bar_free, t == 1 ? 0u : 1u);
                 };
-                if (has_t1 && j > 0) {
-                    if (!(ok = issue_pv(1, j - 1, look_p, look_next_s0))) break;
-                    release(2 * j - 1);
-                } else {
-                    look_next_s0();
+                auto look_p = [&](int t, int i) {
+                    const int j = tile(t, i);
+                    if (kPair && t == 1) return peek(bar_p(1, 0), (uint32_t)i & 1u);   // V_i is there
+                    return peek(bar_full(1, j), par_full(j), bar_p(t, 0), (uint32_t)i & 1u);
+                };
+                auto issue_s = [&](int t, int i) {
+                    tc_fence_after_sync();
+                    const int j = tile(t, i);
+                    const uint64_t q = t == 0 ? q0_desc : q1_desc, k = k_desc0 + slot_off16(j);
+                    if constexpr (kPieces == 2) umma_ss_x8(tmem + kColS, q, k, idesc_s);
+                    else umma_ss_x4(tmem + kColS, q, k, idesc_s);
+                    umma_commit(smem_u32(&ctl->s_full[t]));
+                    if (t == 1 || !kPair) release(0, j);
+                };
+                // O_t (+)= P_t V_j, half by half as the softmax group hands P over; `next` takes the look at what follows.
+                auto issue_pv = [&](int t, int i, const Look& first, auto&& next) -> bool {
+                    const int j = tile(t, i);
+                    const uint32_t d = tmem + (t == 0 ? kColO0 : kColO1), a = tmem + (t == 0 ? kColP0 : kColP1);
+                    const uint64_t v = v_desc0 + slot_off16(j);
+                    if (!finish(first)) return false;
+                    const Look half = peek(bar_p(t, 1), (uint32_t)i & 1u);
+                    tc_fence_after_sync();
+                    umma_ts_x4(d, a, v, idesc_o, i > 0 ? 1u : 0u);
+                    if (!finish(half)) return false;
+                    next();
+                    tc_fence_after_sync();
+                    umma_ts_x4(d, a + 32, v + 4 * (2048 >> 4), idesc_o, 1u);
+                    umma_commit(smem_u32(&ctl->pv_done[t]));
+                    if (t == 1 || !kPair) release(1, j);
+                    return true;
+                };
+                Look s_look{}, p_look{};
+                if (n0 > 0) {
+                    ok = bars.wait(smem_u32(&ctl->q_full[0]), 0) && bars.wait(bar_full(0, 0), 0);
+                    if (ok) issue_s(0, 0);
+                    if (ok && kPair) ok = bars.wait(smem_u32(&ctl->q_full[1]), 0);
+                    if (n1 > 0) s_look = look_s(1, 0);
                 }
-                if (j + 1 < n_kv) {
-                    if (!(ok = finish(look_s))) break;
+                for (int i = 0; i < n0 && ok; ++i) {
+                    if (i < n1) {
+                        if (!(ok = finish(s_look))) break;
+                        if (i > 0) p_look = look_p(1, i - 1);
+                        issue_s(1, i);
+                    } else if (i > 0 && i - 1 < n1) {
+                        p_look = look_p(1, i - 1);
+                    }
+                    auto look_next_s0 = [&] {
+                        if (i + 1 < n0) s_look = look_s(0, i + 1);
+                    };
+                    if (i > 0 && i - 1 < n1) {
+                        if (!(ok = issue_pv(1, i - 1, p_look, look_next_s0))) break;
+                    } else {
+                        look_next_s0();
+                    }
+                    if (i + 1 < n0) {
+                        if (!(ok = finish(s_look))) break;
+                    }
+                    p_look = look_p(0, i);
+                    if (i + 1 < n0) issue_s(0, i + 1);
+                    if (!(ok = issue_pv(0, i, p_look, [&] { if (i + 1 < n1) s_look = look_s(1, i + 1); }))) break;
                 }
-                look_p = peek(bar_full(2 * j + 1), par_full(2 * j + 1), bar_p(0, 0), (uint32_t)j & 1u);
-                if (j + 1 < n_kv) issue_s(0, j + 1);
-                if (!(ok = issue_pv(0, j, look_p, [&] { if (has_t1) look_s = peek(bar_free, 0u); }))) break;
-                if (!has_t1) release(2 * j + 1);
-            }
-            if (ok && n_kv > 0 && has_t1) {
-                ok = issue_pv(1, n_kv - 1, peek(bar_p(1, 0), (uint32_t)(n_kv - 1) & 1u), [] {});
-                if (ok) release(2 * n_kv - 1);
-            }
+                if (ok && n0 > 0 && n1 == n0) ok = issue_pv(1, n1 - 1, look_p(1, n1 - 1), [] {});
+            };
+            if (pair) run(std::true_type{});
+            else run(std::false_type{});
             if (!ok) {
                 // Leaving early: until the MMAs already issued retire (bounded), so tensor memory is idle when freed.
                 volatile uint32_t never = 0;
@@ -336,23 +362,23 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 mbar_wait(smem_u32(&ctl->drain), 0, &never, 40000000ll);
             }
         }
-    } else if ((warp < 4 && any) || has_t1) {
-        // ------------------------------ softmax of tile 0 / 1 ------------------------------
+    } else if (any) {
+        // ------------------------------ softmax groups ------------------------------
         setmaxnreg_inc<208>();
         const int t = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + kColS, tP = tmem + lane_base + (t == 0 ? kColP0 : kColP1);
         const uint32_t tO = tmem + lane_base + (t == 0 ? kColO0 : kColO1);
         const float c = p.scale_log2;
-        const int tok0 = (job.tile0 + t) * per_tile, rows = min(per_tile, job.s.n_new - tok0) * p.group;
+        const int tok0 = (job.tile0 + (pair ? t : 0)) * per_tile, rows = min(per_tile, job.s.n_new - tok0) * p.group;
         constexpr int kChunks = D / 8;                  // 16-byte chunks of a row
-        const uint32_t q_tile = smem + kSmemQ + t * kQBytes;
+        const uint32_t q_tile = smem + kSmemQ + (pair ? t : 0) * kQBytes;
         // Row r of a tile is token r / group: by a multiplication (r < 128, group <= 128), a division per row cost more than the row.
         const uint32_t over_group = (65536u + (uint32_t)p.group - 1u) / (uint32_t)p.group;
         auto token_of = [&](int r) { return (int)((uint32_t)r * over_group >> 16); };
         constexpr int kAtOnce = 32 / kChunks;           // rows that a warp reads or writes at once
         const int ch = lane % kChunks, first_row = (warp & 3) * 32 + lane / kChunks;
-        {   // Q rows to shared memory as the MMA reads them: 128-byte pieces, chunks swizzled by row. All loads first.
+        if (t == 0 || pair) {   // Q rows to shared memory as the MMA reads them: 128-byte pieces, chunks swizzled by row. All loads first.
             const T* q = static_cast<const T*>(p.q) + (long long)(job.s.first + tok0) * p.q_stride + (long long)kvh * p.group * D + ch * 8;
             uint4 v[kChunks];
 #pragma unroll
@@ -377,12 +403,13 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         bool ok = true;
         const uint32_t all_boxes = (1u << (kKeys / min(kKeys, 1 << p.page_shift))) - 1u;
 
-        for (int j = 0; j < n_kv; ++j) {
-            ok = mbar_wait(smem_u32(&ctl->s_full[t]), j & 1, abort_flag, wait_limit);
+        const int n = steps(t);
+        for (int i = 0; i < n; ++i) {
+            ok = mbar_wait(smem_u32(&ctl->s_full[t]), i & 1, abort_flag, wait_limit);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after_sync();
-            const int base = key00 + j * kKeys;
+            const int tile = tile_of(t, i), base = key00 + tile * kKeys;
             uint32_t s[128];
             float mx[kMaxChains];
             uint32_t boxes;
@@ -390,14 +417,14 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             auto hide = [&](int from) {                 // scores [from, from + 64) of keys that the row does not see
                 const int first = see.lo - base, end = see.hi - base;
 #pragma unroll
-                for (int i = from; i < from + 64; ++i)
-                    if (i < first || i >= end) s[i] = __float_as_uint(-INFINITY);
+                for (int k = from; k < from + 64; ++k)
+                    if (k < first || k >= end) s[k] = __float_as_uint(-INFINITY);
                 if (boxes != all_boxes) {
 #pragma unroll
-                    for (int i = from; i < from + 64; i += 16)
-                        if (!(boxes >> (i >> min(p.page_shift, 7)) & 1u)) {
+                    for (int k = from; k < from + 64; k += 16)
+                        if (!(boxes >> (k >> min(p.page_shift, 7)) & 1u)) {
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) s[i + k] = __float_as_uint(-INFINITY);
+                            for (int e = 0; e < 16; ++e) s[k + e] = __float_as_uint(-INFINITY);
                         }
                 }
             };
@@ -408,7 +435,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 uint32_t(&s3)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[96]);
                 tmem_ld_x32(tS + 0, s0);
                 tmem_ld_x32(tS + 32, s1);
-                boxes = *reinterpret_cast<volatile uint32_t*>(&ctl->boxes[j % kBoxRing]);
+                boxes = *reinterpret_cast<volatile uint32_t*>(&ctl->boxes[tile % kBoxRing]);
                 masked = __any_sync(0xffffffffu, base < see.lo || base + kKeys > see.hi) || boxes != all_boxes;
                 tmem_wait_ld();
                 tmem_ld_x32(tS + 64, s2);
@@ -423,7 +450,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             if (masked) hide(64);
             row_max64<false>(&s[64], mx);
             const float m_tile = row_max_finish(mx);
-            const bool pv_seen = j == 0 || mbar_test(smem_u32(&ctl->pv_done[t]), (j - 1) & 1);
+            const bool pv_seen = i == 0 || mbar_test(smem_u32(&ctl->pv_done[t]), (i - 1) & 1);
 
             const bool need = (m_tile - m_ref) * c > kLazyThreshold;
             if (__any_sync(0xffffffffu, need)) {
@@ -431,8 +458,8 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 const float f = m_new == -INFINITY ? 1.0f : ex2_approx((m_ref - m_new) * c);
                 l_sum *= f;
                 m_ref = m_new;
-                if (j > 0) {
-                    ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (j - 1) & 1, abort_flag, wait_limit);
+                if (i > 0) {
+                    ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (i - 1) & 1, abort_flag, wait_limit);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after_sync();
@@ -442,7 +469,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                         tmem_ld_x32(tO + q * 32, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
                         tmem_st_x32(tO + q * 32, o);
                     }
                 }
@@ -464,7 +491,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 }
                 exp_chunk<T>(&s[q * 32 + 16], pk + 8, c, neg_mc, sum);
                 if (q == 0 && !__all_sync(0xffffffffu, pv_seen)) {
-                    ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (j - 1) & 1, abort_flag, wait_limit);
+                    ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (i - 1) & 1, abort_flag, wait_limit);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 }
@@ -481,33 +508,82 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         }
 
         // ------------------------------ epilogue ------------------------------
-        if (ok && n_kv > 0) {
-            ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (n_kv - 1) & 1, abort_flag, wait_limit);
+        if (ok && n > 0) {
+            ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (n - 1) & 1, abort_flag, wait_limit);
             ok = __all_sync(0xffffffffu, ok);
         }
-        if (ok) {
+        // Split form: group 1 leaves its rows, in fp32, with their references and sums where the key tiles were (once no MMA reads
+        // them any more), and group 0 takes them in.
+        constexpr uint32_t kShareRow = D * 4 + 16;
+        const uint32_t share = smem + kSmemRing + r * kShareRow;
+        const bool joins = !pair && n_kv > 1;
+        float other = 0.0f;                                  // factor of group 1's row
+        if (ok && joins) {
+            if (t == 1) {
+                ok = mbar_wait(smem_u32(&ctl->pv_done[0]), (steps(0) - 1) & 1, abort_flag, wait_limit);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok) {
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int q = 0; q < D / 32; ++q) {
+                        uint32_t o[32];
+                        tmem_ld_x32(tO + q * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) st_shared_v4(share + (q * 32 + k) * 4, make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]));
+                    }
+                    st_shared_v4(share + D * 4, make_uint4(__float_as_uint(m_ref), __float_as_uint(l_sum), 0u, 0u));
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&ctl->joined));
+                }
+            } else {
+                ok = mbar_wait(smem_u32(&ctl->joined), 0, abort_flag, wait_limit);
+                ok = __all_sync(0xffffffffu, ok);
+            }
+        }
+        if (ok && (t == 0 || pair)) {
             tc_fence_after_sync();
+            float mine = 1.0f;
+            if (joins) {
+                const uint4 v = ld_shared_v4(share + D * 4);
+                const float m1 = __uint_as_float(v.x), m = fmaxf(m_ref, m1);
+                if (m != -INFINITY) {
+                    mine = ex2_approx((m_ref - m) * c);
+                    other = ex2_approx((m1 - m) * c);
+                }
+                l_sum = l_sum * mine + __uint_as_float(v.y) * other;
+                m_ref = m;
+            }
             const bool none = l_sum == 0.0f && m_ref == -INFINITY;      // a row that sees no key is zero
             const float inv = 1.0f / l_sum;
+            mine *= inv;
+            other *= inv;
             // Rows go out through the shared memory of the tile's Q (no MMA reads it any more), a bulk copy each: 16-byte stores by
             // half-warps kept the CTA 6000 to 7000 clk.
             const uint32_t park = q_tile + r * (D * 2 + 16);
 #pragma unroll
             for (int q = 0; q < D / 32; ++q) {
                 uint32_t o[32];
-                if (n_kv > 0) {
+                if (n > 0) {
                     tmem_ld_x32(tO + q * 32, o);
                     tmem_wait_ld();
                 }
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    uint4 v;
-                    v.x = Half16<T>::pack(__uint_as_float(o[i + 0]) * inv, __uint_as_float(o[i + 1]) * inv);
-                    v.y = Half16<T>::pack(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-                    v.z = Half16<T>::pack(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-                    v.w = Half16<T>::pack(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                for (int k = 0; k < 32; k += 8) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(o[k + e]) * mine;
+                    if (joins) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 4) {
+                            const uint4 w = ld_shared_v4(share + (q * 32 + k + e) * 4);
+                            x[e] += __uint_as_float(w.x) * other, x[e + 1] += __uint_as_float(w.y) * other;
+                            x[e + 2] += __uint_as_float(w.z) * other, x[e + 3] += __uint_as_float(w.w) * other;
+                        }
+                    }
+                    uint4 v = make_uint4(Half16<T>::pack(x[0], x[1]), Half16<T>::pack(x[2], x[3]), Half16<T>::pack(x[4], x[5]), Half16<T>::pack(x[6], x[7]));
                     if (none) v = make_uint4(0, 0, 0, 0);
-                    st_shared_v4(park + (q * 4 + (i >> 3)) * 16, v);
+                    st_shared_v4(park + (q * 4 + (k >> 3)) * 16, v);
                 }
             }
             fence_proxy_async_smem();
