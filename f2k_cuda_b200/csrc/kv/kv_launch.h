@@ -17,8 +17,8 @@ cudaError_t paged_token_prepare(PagedType type, PagedType cache, int head_dim); 
 cudaError_t paged_token_launch(const AttendParams& p, PagedType type, PagedType cache, int head_dim, int rows, int used_rows,
                                cudaStream_t stream);
 
-// Prompts, 16-bit caches; max_new: the most new tokens of a sequence, sms: of the device. No workspace.
-cudaError_t paged_prompt_prepare(PagedType type, int head_dim);
-cudaError_t paged_prompt_launch(const AttendParams& p, PagedType type, int head_dim, int max_new, int sms, cudaStream_t stream);
+// Prompts; max_new: the most new tokens of a sequence, sms: of the device. No workspace.
+cudaError_t paged_prompt_prepare(PagedType type, PagedType cache, int head_dim);
+cudaError_t paged_prompt_launch(const AttendParams& p, PagedType type, PagedType cache, int head_dim, int max_new, int sms, cudaStream_t stream);
 
 }  // namespace f2k

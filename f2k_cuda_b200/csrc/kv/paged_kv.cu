@@ -106,9 +106,9 @@ Workspace workspace_of(const f2k_kv* h, int rows) {
     return w;
 }
 int group_of(const f2k_kv* h) { return h->cfg.n_heads / h->cfg.n_kv_heads; }
-// Which kernel attends. An e4m3 cache has the token kernel only: its products are fp16 ones on registers.
+// Which kernel attends.
 bool takes_prompt_kernel(const f2k_kv* h, const f2k_kv_batch* b) {
-    return h->cfg.cache_type != F2K_E4M3 && b->max_new > 1 && (long long)b->max_new * group_of(h) > 64;
+    return b->max_new > 1 && (long long)b->max_new * group_of(h) > 64;
 }
 int rows_of(const f2k_kv* h, const f2k_kv_batch* b) { return token_rows((long long)b->max_new * group_of(h)); }
 
@@ -165,13 +165,13 @@ int f2k_kv_create(const f2k_kv_config* cfg, f2k_kv** out) {
     if (e != cudaSuccess) return fail_cuda(h, "cudaDeviceGetAttribute", e);
     if (major != 10) return fail(h, F2K_ERR_UNSUPPORTED, "this library contains sm_100a code only (needs a B200-class GPU)");
     e = paged_token_prepare((PagedType)c.type, (PagedType)c.cache_type, c.head_dim);
-    if (e == cudaSuccess && c.cache_type != F2K_E4M3) e = paged_prompt_prepare((PagedType)c.type, c.head_dim);
+    if (e == cudaSuccess) e = paged_prompt_prepare((PagedType)c.type, (PagedType)c.cache_type, c.head_dim);
     if (e != cudaSuccess) return fail_cuda(h, "kernel load", e);
     const int unit = token_unit_keys(c.head_dim * (c.cache_type == F2K_E4M3 ? 1 : 2));
     const int rows = unit < c.page_size ? unit : c.page_size;
     int rc = encode_pages(h, &h->token_k, c.k_pages, c.k_page_stride, c.k_head_stride, c.k_token_stride, rows, 0);
     if (rc == F2K_OK) rc = encode_pages(h, &h->token_v, c.v_pages, c.v_page_stride, c.v_head_stride, c.v_token_stride, rows, 0);
-    if (rc == F2K_OK && c.cache_type != F2K_E4M3) {
+    if (rc == F2K_OK) {
         const int most = c.page_size < kPromptTile ? c.page_size : kPromptTile;
         rc = encode_pages(h, &h->prompt_k, c.k_pages, c.k_page_stride, c.k_head_stride, c.k_token_stride, most, 1);
         if (rc == F2K_OK) rc = encode_pages(h, &h->prompt_v, c.v_pages, c.v_page_stride, c.v_head_stride, c.v_token_stride, most, 1);
@@ -246,7 +246,7 @@ int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const void* q, void* o, 
     if (takes_prompt_kernel(h, batch)) {
         p.tm_k = h->prompt_k;
         p.tm_v = h->prompt_v;
-        const cudaError_t e = paged_prompt_launch(p, (PagedType)c.type, c.head_dim, batch->max_new, h->sms, static_cast<cudaStream_t>(stream));
+        const cudaError_t e = paged_prompt_launch(p, (PagedType)c.type, (PagedType)c.cache_type, c.head_dim, batch->max_new, h->sms, static_cast<cudaStream_t>(stream));
         return e == cudaSuccess ? F2K_OK : fail_cuda(h, "attention launch", e);
     }
     const int rows = rows_of(h, batch);

@@ -1,4 +1,4 @@
-// Causal attention of prompts over a paged cache, 16-bit types, head_dim 64 or 128, for sm_100a.
+// Causal attention of prompts over a paged cache, head_dim 64 or 128, for sm_100a.
 //
 // A tile is 128 query rows of one sequence and key head: 128 / group new tokens with the `group` query heads of the key
 // head side by side (fewer rows where group does not divide 128), so a key and its value are read once for all heads
@@ -22,6 +22,11 @@
 //    window. K and V have a ring and a loader each: K of the tile after next may come in as soon as S is done with its slot.
 //  * Q is fetched by the softmax groups themselves (the rows of a tile are a gather once group is not a power of two).
 //  * Scores are masked by key number, only in tiles that some row of the warp does not see whole.
+//
+// e4m3 caches: a tile comes in as bytes into the second half of its slot, and its loader turns it into fp16 (exactly) in place,
+// row by row, before it hands it over; rows of V to be cleared are written as zeros then. The products are fp16 ones; bf16
+// queries are brought into fp16's range by a power of two per row, which goes into the row's exponent factor with the
+// head's scale of K. The token kernel, which converts in registers for every 64 rows anew, took 6.6 ms for 8192 tokens.
 //
 // Long tiles first: the grid's first CTAs are the last tiles of every sequence, which see the most keys.
 #include "../attn_params.h"
@@ -60,6 +65,7 @@ struct Ctl {
     uint64_t joined;                                    // split form: group 1 has left its share (these: four arrivals each)
     uint64_t full[2][kMostStages];                      // [K, V][slot]
     uint64_t empty[2][kMostStages];
+    uint64_t raw[2][kMostStages];                       // e4m3: the bytes are there
     uint64_t s_full[2];
     uint64_t pv_done[2];
     uint64_t drain;
@@ -67,6 +73,7 @@ struct Ctl {
     uint32_t tmem_base;
     uint32_t abort;
     uint32_t boxes[kBoxRing];                           // pages of a key tile that were fetched, a bit each
+    float row_scale[2][kRows];                          // e4m3 with bf16 queries: what a row of S is multiplied by
 };
 
 struct WarpBarriers {                                   // the MMA warp's side of barrier_look.h
@@ -141,14 +148,27 @@ constexpr uint32_t kQArea = kRows * (D * 2 + 16);
 template <int D>
 constexpr int kSmemBytes = 2 * (int)kQArea<D> + 2 * kStages<D> * (D / 64) * (int)kPieceBytes + 1024;
 
-template <class T, int D>
+// One row of e4m3, LPR lanes of 16 bytes, to fp16: lane c writes elements 16c .. 16c + 15 of the row.
+struct Row16 {
+    uint4 lo, hi;
+};
+__device__ __forceinline__ Row16 f16_of_e4m3x16(const uint4& v) {
+    Row16 r;
+    r.lo = make_uint4(f16x2_of_e4m3x2(v.x), f16x2_of_e4m3x2(v.x >> 16), f16x2_of_e4m3x2(v.y), f16x2_of_e4m3x2(v.y >> 16));
+    r.hi = make_uint4(f16x2_of_e4m3x2(v.z), f16x2_of_e4m3x2(v.z >> 16), f16x2_of_e4m3x2(v.w), f16x2_of_e4m3x2(v.w >> 16));
+    return r;
+}
+
+template <class T, bool kE4m3, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     constexpr int kPieces = D / 64;                     // 128-byte pieces of a row
     constexpr uint32_t kTileBytes = kPieces * kPieceBytes;
     constexpr int kSlots = kStages<D>;
     constexpr uint32_t kQBytes = kQArea<D>, kSmemQ = 0, kSmemRing = 2 * kQBytes;      // K slots, then V slots
-    constexpr uint32_t kFormat = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+    using M = std::conditional_t<kE4m3, __half, T>;     // the type of the products
+    constexpr uint32_t kFormat = std::is_same_v<M, __nv_bfloat16> ? 1u : 0u;
+    constexpr uint32_t kRowBytes = kE4m3 ? D : 128;     // of a piece as it comes in
     extern __shared__ uint8_t smem_raw[];
     __shared__ Ctl ctl_;
     Ctl* ctl = &ctl_;
@@ -162,8 +182,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     grid_launch_dependents();
     if (warp == kLoadK) {
         constexpr int kBars = offsetof(Ctl, tmem_base) / sizeof(uint64_t), kPerWarp = offsetof(Ctl, full) / sizeof(uint64_t);
-        static_assert(kBars <= 32, "a lane per barrier");
-        if (lane < kBars) mbar_init(smem_u32(ctl) + lane * 8, lane < kPerWarp ? 4 : 1);    // a group's four warps arrive, or one thread
+        for (int i = lane; i < kBars; i += 32) mbar_init(smem_u32(ctl) + i * 8, i < kPerWarp ? 4 : 1);    // a group's four warps arrive, or one thread
         if (lane == 0) ctl->abort = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
@@ -202,7 +221,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             const int kv = warp == kLoadK ? 0 : 1;
             const int box_rows = min(kKeys, 1 << p.page_shift), n_boxes = kKeys / box_rows;
             const int box = lane & 7, piece = lane >> 3;
-            const bool mine = box < n_boxes && piece < kPieces;
+            const bool mine = box < n_boxes && piece < (kE4m3 ? 1 : kPieces);
             const uint32_t all_boxes = (1u << n_boxes) - 1u;
             const int32_t* row = p.batch.table + (any ? job.b : 0) * p.batch.table_stride;
             const CUtensorMap* map = kv == 0 ? &p.tm_k : &p.tm_v;
@@ -211,6 +230,45 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 return mine && j < n_kv && k < hi && k + box_rows > lo;
             };
             auto look_up = [&](int j) { return needed(j) ? row[(key00 + j * kKeys + box * box_rows) >> p.page_shift] : 0; };
+            // e4m3: tile j, which has come in, to fp16 where it lies. Rows go up: what row r's 256 (128) bytes of fp16 are written over has
+            // been read before (its own bytes, or rows below it).
+            auto convert = [&](int j, uint32_t boxes) -> bool {
+                const int slot = j % kSlots, base = key00 + j * kKeys;
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->raw[kv][slot]), (j / kSlots) & 1, abort_flag, wait_limit))) return false;
+                const bool clear = kv == 1 && (base < lo || base + kKeys > hi || boxes != all_boxes);
+                const uint32_t dst = smem + kSmemRing + (kv * kSlots + slot) * kTileBytes, in = dst + kTileBytes / 2;
+                constexpr int kLanes = D / 16, kAtOnce = 32 / kLanes, kBatch = 4;      // lanes of a row, rows of the warp at once
+                const int ch = lane % kLanes;
+#pragma unroll 1
+                for (int r0 = lane / kLanes; r0 < kKeys; r0 += kAtOnce * kBatch) {
+                    uint4 v[kBatch];
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) {
+                        const int r = r0 + u * kAtOnce, twist = D == 128 ? (r & 7) : ((r >> 1) & 3);
+                        v[u] = ld_shared_v4(in + r * D + ((ch ^ twist) << 4));
+                        if (clear) {
+                            const int key = base + r;
+                            if (!(key >= lo && key < hi && (boxes >> (r / box_rows) & 1u))) v[u] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) {
+                        const int r = r0 + u * kAtOnce;
+                        const Row16 w = f16_of_e4m3x16(v[u]);
+                        const uint32_t at = dst + (ch >> 2) * kPieceBytes + r * 128;
+                        st_shared_v4(at + (((2 * ch & 7) ^ (r & 7)) << 4), w.lo);
+                        st_shared_v4(at + (((2 * ch + 1 & 7) ^ (r & 7)) << 4), w.hi);
+                    }
+                    __syncwarp();
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->full[kv][slot]));
+                return true;
+            };
+            uint32_t came_boxes = 0;                          // e4m3: of the tile that is to be converted next
+            int converted = 0;
             int next_page = look_up(0), cleaned = 0, j = 0;
             bool ok = true;
             for (; j < n_kv; ++j) {
@@ -219,22 +277,39 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 const bool wanted = needed(j), good = wanted && (unsigned)page < (unsigned)p.n_pages;
                 if (wanted && !good) atomicOr(p.status, (int)kStatusBadPage);
                 const uint32_t boxes = __ballot_sync(0xffffffffu, good) & 0xFFu;
+                if constexpr (kE4m3) {
+                    // The tile before is converted while this one's slot is still in use, or its copy on its way.
+                    const bool free = j < kSlots || mbar_test(smem_u32(&ctl->empty[kv][slot]), ((j / kSlots) & 1) ^ 1u);
+                    if (converted < j && !__all_sync(0xffffffffu, free)) {
+                        if (!(ok = convert(converted, came_boxes))) break;
+                        ++converted;
+                    }
+                }
                 if (j >= kSlots) {
                     ok = mbar_wait(smem_u32(&ctl->empty[kv][slot]), ((j / kSlots) & 1) ^ 1u, abort_flag, wait_limit);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 }
                 const bool clear = kv == 1 && (base < lo || base + kKeys > hi || boxes != all_boxes);
-                const uint32_t full = smem_u32(&ctl->full[kv][slot]), bar = clear ? smem_u32(&ctl->clean) : full;
-                const uint32_t dst = smem + kSmemRing + (kv * kSlots + slot) * kTileBytes;
+                const uint32_t full = smem_u32(&ctl->full[kv][slot]);
+                const uint32_t bar = kE4m3 ? smem_u32(&ctl->raw[kv][slot]) : clear ? smem_u32(&ctl->clean) : full;
+                const uint32_t dst = smem + kSmemRing + (kv * kSlots + slot) * kTileBytes, in = dst + (kE4m3 ? kTileBytes / 2 : 0);
                 if (lane == 0) {
                     if (kv == 0) ctl->boxes[j % kBoxRing] = boxes;
-                    mbar_arrive_expect_tx(bar, (uint32_t)__popc(boxes) * kPieces * (uint32_t)box_rows * 128u);
+                    mbar_arrive_expect_tx(bar, (uint32_t)__popc(boxes) * (kE4m3 ? 1 : kPieces) * (uint32_t)box_rows * kRowBytes);
                 }
                 __syncwarp();
                 if (good) {
                     const int first = (base + box * box_rows) & ((1 << p.page_shift) - 1);
-                    tma_load_5d(dst + piece * kPieceBytes + box * box_rows * 128, map, bar, 0, first, piece, kvh, page);
+                    tma_load_5d(in + piece * kPieceBytes + box * box_rows * kRowBytes, map, bar, 0, first, piece, kvh, page);
+                }
+                if constexpr (kE4m3) {
+                    if (converted < j) {
+                        if (!(ok = convert(converted, came_boxes))) break;
+                        ++converted;
+                    }
+                    came_boxes = boxes;
+                    continue;
                 }
                 if (clear) {
                     ok = mbar_wait(bar, cleaned & 1, abort_flag, wait_limit);
@@ -252,12 +327,13 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                     if (lane == 0) mbar_arrive(full);
                 }
             }
+            if (kE4m3 && ok && converted < n_kv) ok = convert(converted, came_boxes);
             if (!ok) {
                 // Leaving early: let the copies this warp started land first (bounded).
                 volatile uint32_t never = 0;
-                if (kv == 1) mbar_wait(smem_u32(&ctl->clean), cleaned & 1, &never, 4000000ll);
+                if (kv == 1 && !kE4m3) mbar_wait(smem_u32(&ctl->clean), cleaned & 1, &never, 4000000ll);
                 for (int i = max(0, j - kSlots); i < j; ++i)
-                    mbar_wait(smem_u32(&ctl->full[kv][i % kSlots]), (i / kSlots) & 1, &never, 40000000ll);
+                    mbar_wait(smem_u32(kE4m3 ? &ctl->raw[kv][i % kSlots] : &ctl->full[kv][i % kSlots]), (i / kSlots) & 1, &never, 40000000ll);
             }
         } else if (warp == kMmaWarp) {
             // ------------------------------ MMA issuer, converged ------------------------------
@@ -369,7 +445,8 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + kColS, tP = tmem + lane_base + (t == 0 ? kColP0 : kColP1);
         const uint32_t tO = tmem + lane_base + (t == 0 ? kColO0 : kColO1);
-        const float c = p.scale_log2;
+        float c = p.scale_log2;                         // of this thread's row
+        if (kE4m3 && p.k_scale != nullptr) c *= p.k_scale[kvh];
         const int tok0 = (job.tile0 + (pair ? t : 0)) * per_tile, rows = min(per_tile, job.s.n_new - tok0) * p.group;
         constexpr int kChunks = D / 8;                  // 16-byte chunks of a row
         const uint32_t q_tile = smem + kSmemQ + (pair ? t : 0) * kQBytes;
@@ -387,6 +464,25 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 v[i] = make_uint4(0, 0, 0, 0);
                 if (r < rows) v[i] = *reinterpret_cast<const uint4*>(q + tok * p.q_stride + (r - tok * p.group) * D);
             }
+            if constexpr (kE4m3 && std::is_same_v<T, __nv_bfloat16>) {
+                // the largest element of a row into [2^14, 2^15); an infinite one is left as it is
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i) {
+                    using H = Half16<T>;
+                    uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                    float top = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(H::lo(w[k])), fabsf(H::hi(w[k]))));
+#pragma unroll
+                    for (int d = 1; d < kChunks; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const unsigned e = __float_as_uint(top) >> 23, f = e == 255u ? 127u : min(253u, 268u - e);
+                    const float up = __uint_as_float(f << 23);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = Half16<M>::pack(H::lo(w[k]) * up, H::hi(w[k]) * up);
+                    v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (ch == 0) ctl->row_scale[t][first_row + i * kAtOnce] = __uint_as_float((254u - f) << 23);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
                 const int r = first_row + i * kAtOnce;
@@ -400,6 +496,14 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         KeyRange see{0, 0x7fffffff};                    // of this thread's row; rows that do not exist are not masked
         if (r < rows) see = visible_keys(job.s, tok0 + token_of(r), p.window);
         float m_ref = -INFINITY, l_sum = 0.0f;
+        if constexpr (kE4m3 && std::is_same_v<T, __nv_bfloat16>) {
+            if (t == 1 && !pair) {                      // the rows are group 0's
+                const bool came = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->q_full[0]), 0, abort_flag, wait_limit));
+                if (came) c *= ctl->row_scale[0][r];
+            } else {
+                c *= ctl->row_scale[t][r];              // written by this warp in front of the __syncwarp above
+            }
+        }
         bool ok = true;
         const uint32_t all_boxes = (1u << (kKeys / min(kKeys, 1 << p.page_shift))) - 1u;
 
@@ -481,7 +585,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 uint32_t pk[16];
-                exp_chunk<T>(&s[q * 32], pk, c, neg_mc, sum);
+                exp_chunk<M>(&s[q * 32], pk, c, neg_mc, sum);
                 if (pending >= 0) {
                     tmem_wait_st();
                     tc_fence_before_sync();
@@ -489,7 +593,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                     if (lane == 0) mbar_arrive(smem_u32(&ctl->p_full[t][0]) + pending * 8);
                     pending = -1;
                 }
-                exp_chunk<T>(&s[q * 32 + 16], pk + 8, c, neg_mc, sum);
+                exp_chunk<M>(&s[q * 32 + 16], pk + 8, c, neg_mc, sum);
                 if (q == 0 && !__all_sync(0xffffffffu, pv_seen)) {
                     ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (i - 1) & 1, abort_flag, wait_limit);
                     ok = __all_sync(0xffffffffu, ok);
@@ -555,7 +659,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 m_ref = m;
             }
             const bool none = l_sum == 0.0f && m_ref == -INFINITY;      // a row that sees no key is zero
-            const float inv = 1.0f / l_sum;
+            const float inv = (kE4m3 && p.v_scale != nullptr ? p.v_scale[kvh] : 1.0f) / l_sum;
             mine *= inv;
             other *= inv;
             // Rows go out through the shared memory of the tile's Q (no MMA reads it any more), a bulk copy each: 16-byte stores by
@@ -608,42 +712,46 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     }
 }
 
+// f(type, e4m3, dim) for the run-time choice.
 template <class F>
-cudaError_t with_types(PagedType type, int head_dim, F&& f) {
-    auto by_dim = [&](auto t) { return head_dim == 64 ? f(t, std::integral_constant<int, 64>{}) : f(t, std::integral_constant<int, 128>{}); };
-    return type == kBf16 ? by_dim(__nv_bfloat16{}) : by_dim(__half{});
+cudaError_t with_types(PagedType type, PagedType cache, int head_dim, F&& f) {
+    auto by_dim = [&](auto t, auto e) {
+        return head_dim == 64 ? f(t, e, std::integral_constant<int, 64>{}) : f(t, e, std::integral_constant<int, 128>{});
+    };
+    auto by_cache = [&](auto t) { return cache == kE4m3 ? by_dim(t, std::true_type{}) : by_dim(t, std::false_type{}); };
+    return type == kBf16 ? by_cache(__nv_bfloat16{}) : by_cache(__half{});
 }
 
 }  // namespace
 
-cudaError_t paged_prompt_prepare(PagedType type, int head_dim) {
-    return with_types(type, head_dim, [](auto t, auto d) {
-        return cudaFuncSetAttribute(paged_prompt_kernel<decltype(t), decltype(d)::value>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+cudaError_t paged_prompt_prepare(PagedType type, PagedType cache, int head_dim) {
+    return with_types(type, cache, head_dim, [](auto t, auto e, auto d) {
+        return cudaFuncSetAttribute(paged_prompt_kernel<decltype(t), decltype(e)::value, decltype(d)::value>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     kSmemBytes<decltype(d)::value>);
     });
 }
 
-cudaError_t paged_prompt_launch(const AttendParams& p, PagedType type, int head_dim, int max_new, int sms, cudaStream_t stream) {
-    return with_types(type, head_dim, [&](auto t, auto d) {
-        // CTAs that the sequences can need: their tiles rounded up, whatever the lengths.
-        const int per_tile = kRows / p.group;
-        auto ctas = [&](int per_cta) {
-            const long long step = (long long)per_tile * per_cta;
-            const long long by_tokens = p.batch.n_tokens / step + p.batch.n_seqs, by_most = (max_new + step - 1) / step * p.batch.n_seqs;
-            return (by_tokens < by_most ? by_tokens : by_most) * p.n_kv_heads;
-        };
-        const int per_cta = ctas(2) >= sms ? 2 : 1;
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)ctas(per_cta));
-        cfg.blockDim = dim3(kThreads);
+cudaError_t paged_prompt_launch(const AttendParams& p, PagedType type, PagedType cache, int head_dim, int max_new, int sms, cudaStream_t stream) {
+    // CTAs that the sequences can need: their tiles rounded up, whatever the lengths.
+    const int per_tile = kRows / p.group;
+    auto ctas = [&](int per_cta) {
+        const long long step = (long long)per_tile * per_cta;
+        const long long by_tokens = p.batch.n_tokens / step + p.batch.n_seqs, by_most = (max_new + step - 1) / step * p.batch.n_seqs;
+        return (by_tokens < by_most ? by_tokens : by_most) * p.n_kv_heads;
+    };
+    const int per_cta = ctas(2) >= sms ? 2 : 1;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas(per_cta));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return with_types(type, cache, head_dim, [&](auto t, auto e, auto d) {
         cfg.dynamicSmemBytes = kSmemBytes<decltype(d)::value>;
-        cfg.stream = stream;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, paged_prompt_kernel<decltype(t), decltype(d)::value>, p, per_cta);
+        return cudaLaunchKernelEx(&cfg, paged_prompt_kernel<decltype(t), decltype(e)::value, decltype(d)::value>, p, per_cta);
     });
 }
 

@@ -85,11 +85,11 @@ PROMPTS = [([64], [64]), ([128], [128]), ([33], [33]), ([300], [300]), ([129, 0,
 
 
 @pytest.mark.parametrize("news,lens", PROMPTS, ids=[str(i) for i in range(len(PROMPTS))])
-@pytest.mark.parametrize("dtype", [BF, HF], ids=ids)
+@pytest.mark.parametrize("dtype,cache", TYPES, ids=ids)
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,kv_heads,page", [(8, 2, 16), (2, 2, 64), (3, 1, 128), (14, 2, 32), (4, 1, 256)])
-def test_prompts(news, lens, dtype, dim, heads, kv_heads, page):
-    p = Problem(news, lens, heads, kv_heads, dim, page, dtype, pad=5, gap=8, seed=sum(lens) + dim + heads)
+def test_prompts(news, lens, dtype, cache, dim, heads, kv_heads, page):
+    p = Problem(news, lens, heads, kv_heads, dim, page, dtype, cache, scales=cache is E4, pad=5, gap=8, seed=sum(lens) + dim + heads)
     p.o.fill_(9.0)
     p.attend()
     p.check_attend()
@@ -98,10 +98,10 @@ def test_prompts(news, lens, dtype, dim, heads, kv_heads, page):
 
 
 @pytest.mark.parametrize("window", [1, 50, 128, 300])
-@pytest.mark.parametrize("heads,dim,page", [(4, 128, 16), (2, 64, 128), (12, 128, 64)])
-def test_prompts_with_a_window(window, heads, dim, page):
+@pytest.mark.parametrize("heads,dim,page,cache", [(4, 128, 16, BF), (2, 64, 128, BF), (12, 128, 64, BF), (4, 128, 32, E4), (6, 64, 16, E4)], ids=ids)
+def test_prompts_with_a_window(window, heads, dim, page, cache):
     """Pages in front of the window are gone: their entries in the table are outside the cache."""
-    p = Problem([500, 40, 130], [500, 900, 700], heads, 2, dim, page, BF, window=window, seed=window)
+    p = Problem([500, 40, 130], [500, 900, 700], heads, 2, dim, page, BF, cache, window=window, seed=window)
     for b, (n, m) in enumerate(zip(p.news, p.lens)):
         gone = max(0, m - n + 1 - window) // page
         p.table[b, :gone] = -1
@@ -109,15 +109,16 @@ def test_prompts_with_a_window(window, heads, dim, page):
     assert p.kv.device_status() == 0
     p.table = p.table.clamp(min=0)                      # any page: the formula masks those keys
     for pages in (p.k_pages, p.v_pages):
-        pages.nan_to_num_(0.0)
+        pages.copy_(pages.float().nan_to_num(0.0).to(pages.dtype))
     p.check_attend()
 
 
-def test_many_prompts_two_tiles_a_cta():
-    p = Problem([700, 513, 650, 40, 0, 333], [700, 513, 1200, 40, 3, 2000], 32, 8, 128, 16, BF, seed=21)
+@pytest.mark.parametrize("cache", [None, E4], ids=ids)
+def test_many_prompts_two_tiles_a_cta(cache):
+    p = Problem([700, 513, 650, 40, 0, 333], [700, 513, 1200, 40, 3, 2000], 32, 8, 128, 16, BF, cache, seed=21)
     p.attend()
     p.check_attend()
-    p = Problem([700, 513, 650], [700, 513, 1200], 30, 10, 64, 16, HF, seed=22)
+    p = Problem([700, 513, 650], [700, 513, 1200], 30, 10, 64, 16, HF, cache, seed=22)
     p.attend()
     p.check_attend()
 
@@ -138,8 +139,10 @@ def test_prompts_with_fewer_keys_than_tokens():
     p.check_attend()
 
 
-def test_prompt_with_a_page_outside_the_cache():
-    p = Problem([150], [400], 4, 2, 128, 32, HF, seed=25)
+@pytest.mark.parametrize("cache", [HF, E4], ids=ids)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_with_a_page_outside_the_cache(cache, dim):
+    p = Problem([150], [400], 4, 2, dim, 32, HF, cache, seed=25)
     whole = [p.keys(0, x) for x in (p.k_pages, p.v_pages)]
     p.table[0, 3] = 10 ** 6                             # keys 96 .. 127
     p.attend()
