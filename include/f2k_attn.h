@@ -450,7 +450,8 @@ int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const void* q, const voi
                   const void* gamma_q, const void* gamma_k, const float* cos_table, const float* sin_table,
                   int n_positions, float eps, void* q_out, const f2k_kv_strides* strides, void* stream);
 
-/* Bytes of workspace that f2k_kv_attend needs for a batch with this max_new (0 for prompts). Calls whose GPU work may overlap need one each. */
+/* Bytes of workspace that f2k_kv_attend needs for a batch of this n_seqs and max_new (0 for prompts).
+ * Calls whose GPU work may overlap need one each. */
 size_t f2k_kv_workspace_bytes(const f2k_kv* h, const f2k_kv_batch* batch);
 
 /* o = softmax(scale q K^T) V over the keys that each token sees; zero for a token that sees none.
