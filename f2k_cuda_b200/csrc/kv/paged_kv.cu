@@ -100,7 +100,7 @@ Workspace workspace_of(const f2k_kv* h, int rows) {
     Workspace w;
     const size_t ctas = token_ctas(h->sms), shares = 2 * ctas;
     w.join = 0;
-    w.ml = up(sizeof(int4) * ctas);
+    w.ml = up(sizeof(JoinJob) * ctas);
     w.o = w.ml + up(shares * rows * sizeof(float2));
     w.bytes = w.o + shares * rows * h->cfg.head_dim * sizeof(float);
     return w;
@@ -269,7 +269,7 @@ int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const void* q, void* o, 
     if (tiles * c.n_kv_heads * (double)(keys / unit + 1 + kWorkCost) >= 4294967295.0)
         return fail(h, F2K_ERR_UNSUPPORTED, "the batch could hold 2^32 pieces of work: make two calls of it");
     uint8_t* w = static_cast<uint8_t*>(workspace);
-    p.ws_join = reinterpret_cast<int4*>(w + ws.join);
+    p.ws_join = reinterpret_cast<JoinJob*>(w + ws.join);
     p.ws_ml = reinterpret_cast<float2*>(w + ws.ml);
     p.ws_o = reinterpret_cast<float*>(w + ws.o);
     p.n_ctas = token_ctas(h->sms);

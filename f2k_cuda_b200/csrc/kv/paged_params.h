@@ -100,6 +100,12 @@ struct AppendParams {
     int* status;
 };
 
+// What the join does for the cut in front of a CTA's piece: the shares of n pieces (0: nothing), for `rows` query rows of one
+// key head from row0 on of the sequence whose first new token is `first`.
+struct alignas(16) JoinJob {
+    int n, first, kvh, row0, rows, unused[3];
+};
+
 struct AttendParams {
     CUtensorMap tm_k, tm_v;       // [pages][kv heads][128-byte pieces of a row][page][piece]
     PagedBatch batch;
@@ -113,7 +119,7 @@ struct AttendParams {
     long long wait_limit_clk;
     int* status;
     // token kernel: descriptors of joins, then maxima and sums, then unnormalised rows of the pieces
-    int4* ws_join;
+    JoinJob* ws_join;
     float2* ws_ml;
     float* ws_o;
     int n_ctas;

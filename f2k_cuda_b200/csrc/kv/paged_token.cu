@@ -125,7 +125,7 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
     const int n_pieces = pieces(total, p.n_ctas, kWorkCost + KW);
     const int cta = blockIdx.x;
     if (cta >= n_pieces || total == 0) {
-        if (threadIdx.x == 0) p.ws_join[cta] = make_int4(0, 0, 0, 0);
+        if (threadIdx.x == 0) p.ws_join[cta].n = 0;
         return;
     }
     const unsigned begin = piece_begin(total, n_pieces, cta), end = piece_begin(total, n_pieces, cta + 1);
@@ -205,7 +205,6 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
         ahead.kw = kw;
         ahead.enter(p, seq, begin);
         look_up();
-        for (int i = 0; i < kRing - 1; ++i) fetch();
     }
 
     // ---- work by work
@@ -218,7 +217,8 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
     for (unsigned at = begin; at < end; at = walk.stop) {
         const bool any = walk.begin(p, seq, at);
         const Where& x = walk.x;
-        if (at == begin && threadIdx.x == 0) p.ws_join[cta] = make_int4(x.b, x.kvh, x.rt, shares_to_join(x, total, n_pieces, cta));
+        if (at == begin && threadIdx.x == 0)
+            p.ws_join[cta] = JoinJob{shares_to_join(x, total, n_pieces, cta), x.s.first, x.kvh, x.rt * S::kRows, x.s.n_new * p.group - x.rt * S::kRows, {0, 0, 0}};
         if (!any) break;                                      // the piece ends before the work's first unit
         const int tile_rows = min(S::kRows, x.s.n_new * p.group - x.rt * S::kRows);
         const bool active = rw * 8 * NT < tile_rows;
@@ -276,6 +276,10 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
                 see[nt][h] = i < x.s.n_new ? visible_keys(x.s, i, p.window) : KeyRange{0, 0};
             }
         }
+
+        // The first units are fetched behind the first queries' loads, whose latency and that of the pages' numbers then run together.
+        if (rw == 0 && at == begin)
+            for (int i = 0; i < kRing - 1; ++i) fetch();
 
         float o[NT][kSteps][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -586,51 +590,58 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
     }
 }
 
-// One cut's work: the shares of the pieces c-1, c, ... in the order of their keys. A warp has a row.
+// One cut's work: the shares of the pieces c-1, c, ... in the order of their keys. A warp has a row. No shared memory, so that
+// its blocks fit beside the token kernel's and stand ready when that ends; the shares' rows are asked for together with
+// their maxima.
 template <class T, bool kE4m3, int D>
 __global__ void __launch_bounds__(128)
 paged_join_kernel(const __grid_constant__ AttendParams p, int rows) {
-    extern __shared__ float weights[];                        // [4][n_ctas]
     grid_launch_dependents();
-    grid_dependency_wait();
     const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int4 job = p.ws_join[cta];
-    if (job.w == 0) return;
-    const int row = blockIdx.y * 4 + warp, rr = job.z * rows + row, tok = rr / p.group;
-    const SeqView s = seq_of(p.batch, p.page_shift, job.x);
-    if (tok >= s.n_new) return;
-    auto share = [&](int j) { return share_of(cta - 1 + j, j == 0); };
-    float all = -INFINITY;
-    for (int j = lane; j < job.w; j += 32) all = fmaxf(all, p.ws_ml[share(j) * rows + row].x);
+    const int row = blockIdx.y * 4 + warp;
+    grid_dependency_wait();
+    const JoinJob job = p.ws_join[cta];
+    if (job.n == 0 || row >= min(rows, job.rows)) return;
+    auto share = [&](int j) { return (long long)share_of(cta - 1 + j, j == 0) * rows + row; };
+    constexpr int kCols = D / 32, kAhead = 8;
+    float all = -INFINITY, sum = 0.f, acc[kCols] = {};
+    for (int j0 = 0; j0 < job.n; j0 += 32) {                  // 32 shares at a time, a lane for each one's maximum and sum
+        const int n = min(32, job.n - j0);
+        float2 ml = lane < n ? p.ws_ml[share(j0 + lane)] : make_float2(-INFINITY, 0.f);
+        float top = ml.x;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, d));
-    const float to = all == -INFINITY ? 0.f : all;
-    float sum = 0.f, *w = weights + warp * p.n_ctas;
-    for (int j = lane; j < job.w; j += 32) {
-        const float2 v = p.ws_ml[share(j) * rows + row];
-        const float f = ex2_approx(v.x - to);
-        w[j] = f;
-        sum += v.y * f;
-    }
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float to = fmaxf(all, top), ref = to == -INFINITY ? 0.f : to;
+        const float old = ex2_approx(all - ref), f = ex2_approx(ml.x - ref);
+        all = to;
+        float part = ml.y * f;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    __syncwarp();
-    constexpr int kCols = D / 32;
-    float acc[kCols] = {};
-#pragma unroll 8
-    for (int j = 0; j < job.w; ++j) {
-        const float* src = p.ws_o + ((long long)share(j) * rows + row) * D + lane * kCols;
-        const float f = w[j];
+        for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+        sum = sum * old + part;
 #pragma unroll
-        for (int i = 0; i < kCols; i += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(src + i);
-            acc[i] += f * v.x;
-            acc[i + 1] += f * v.y;
+        for (int i = 0; i < kCols; ++i) acc[i] *= old;
+        for (int j = 0; j < n; j += kAhead) {
+            float2 v[kAhead][kCols / 2];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (j + u < n) {
+                    const float* src = p.ws_o + share(j0 + j + u) * D + lane * kCols;
+#pragma unroll
+                    for (int i = 0; i < kCols / 2; ++i) v[u][i] = reinterpret_cast<const float2*>(src)[i];
+                }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const float w = __shfl_sync(0xffffffffu, f, (j + u) & 31);
+                if (j + u < n) {
+#pragma unroll
+                    for (int i = 0; i < kCols / 2; ++i) acc[2 * i] += w * v[u][i].x, acc[2 * i + 1] += w * v[u][i].y;
+                }
+            }
         }
     }
-    const int head = job.y * p.group + (rr - tok * p.group);
-    const long long t = s.first + tok;
-    const float f = (kE4m3 && p.v_scale ? p.v_scale[job.y] : 1.f) / sum;
+    const int rr = job.row0 + row, tok = rr / p.group, head = job.kvh * p.group + (rr - tok * p.group);
+    const long long t = job.first + tok;
+    const float f = (kE4m3 && p.v_scale ? p.v_scale[job.kvh] : 1.f) / sum;
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + t * p.o_stride + (long long)head * D + lane * kCols);
 #pragma unroll
     for (int i = 0; i < kCols; i += 2) dst[i / 2] = all == -INFINITY ? 0u : Half16<T>::pack(acc[i] * f, acc[i + 1] * f);
@@ -683,7 +694,7 @@ cudaError_t launch(const AttendParams& p, int rows, int used_rows, cudaStream_t 
     if (e != cudaSuccess || p.n_ctas == 1) return e;
     cfg.gridDim = dim3(p.n_ctas, (used_rows + 3) / 4);
     cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = 4 * sizeof(float) * p.n_ctas;
+    cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, kE4m3, D>, p, rows);
 }
 
