@@ -46,11 +46,6 @@ class KvBatch(C.Structure):
                 ("table_stride", C.c_longlong), ("cu_seqlens", C.c_void_p), ("kv_lens", C.c_void_p), ("page_table", C.c_void_p)]
 
 
-class KvStrides(C.Structure):
-    """struct f2k_kv_strides: token strides in elements, 0 = dense"""
-    _fields_ = [(n, C.c_longlong) for n in ("q", "k", "v", "q_out", "o")]
-
-
 def _declare(lib: C.CDLL) -> None:
     vp, i, f, sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
     lib.f2k_attn_create.restype = i
@@ -146,11 +141,11 @@ def _declare(lib: C.CDLL) -> None:
     lib.f2k_kv_last_error.restype = C.c_char_p
     lib.f2k_kv_last_error.argtypes = [vp]
     lib.f2k_kv_append.restype = i
-    lib.f2k_kv_append.argtypes = [vp] * 9 + [i, f, vp, vp, vp]
+    lib.f2k_kv_append.argtypes = [vp] * 4
     lib.f2k_kv_workspace_bytes.restype = sz
     lib.f2k_kv_workspace_bytes.argtypes = [vp, vp]
     lib.f2k_kv_attend.restype = i
-    lib.f2k_kv_attend.argtypes = [vp] * 7 + [sz, vp]
+    lib.f2k_kv_attend.argtypes = [vp] * 4
     lib.f2k_kv_device_status.restype = i
     lib.f2k_kv_device_status.argtypes = [vp, C.POINTER(i)]
     lib.f2k_kv_set_wait_limits.restype = i

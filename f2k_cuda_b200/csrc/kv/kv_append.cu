@@ -258,11 +258,7 @@ kv_append_kernel(const __grid_constant__ AppendParams p) {
 }
 
 template <class T, bool kE4m3, int kDim, bool kInter>
-cudaError_t launch(const AppendParams& p, cudaStream_t stream) {
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return e;
+cudaError_t launch(const AppendParams& p, int sms, cudaStream_t stream) {
     constexpr int kTeams = kBlock / (kDim / 16), kMany = 4;
     const int H = p.n_heads, G = p.n_kv_heads;
     const long long n = p.batch.n_tokens, rows = n * (H + 2 * G), sets = n * ((H + kMany - 1) / kMany + 2 * ((G + kMany - 1) / kMany));
@@ -288,12 +284,12 @@ cudaError_t launch(const AppendParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t kv_append_launch(const AppendParams& p, PagedType type, PagedType cache, int head_dim, cudaStream_t stream) {
+cudaError_t kv_append_launch(const AppendParams& p, PagedType type, PagedType cache, int head_dim, int sms, cudaStream_t stream) {
     auto by_dim = [&](auto t, auto e) {
         using T = decltype(t);
         constexpr bool kE = decltype(e)::value;
-        if (p.interleaved) return head_dim == 64 ? launch<T, kE, 64, true>(p, stream) : launch<T, kE, 128, true>(p, stream);
-        return head_dim == 64 ? launch<T, kE, 64, false>(p, stream) : launch<T, kE, 128, false>(p, stream);
+        if (p.interleaved) return head_dim == 64 ? launch<T, kE, 64, true>(p, sms, stream) : launch<T, kE, 128, true>(p, sms, stream);
+        return head_dim == 64 ? launch<T, kE, 64, false>(p, sms, stream) : launch<T, kE, 128, false>(p, sms, stream);
     };
     auto by_cache = [&](auto t) { return cache == kE4m3 ? by_dim(t, std::true_type{}) : by_dim(t, std::false_type{}); };
     return type == kBf16 ? by_cache(__nv_bfloat16{}) : by_cache(__half{});

@@ -7,7 +7,8 @@
 
 namespace f2k {
 
-cudaError_t kv_append_launch(const AppendParams& p, PagedType type, PagedType cache, int head_dim, cudaStream_t stream);
+// sms: of the device, here and below.
+cudaError_t kv_append_launch(const AppendParams& p, PagedType type, PagedType cache, int head_dim, int sms, cudaStream_t stream);
 
 // Query rows of a work that the token kernel's variants hold: 8, 16, 32 or 64; and the CTAs it runs with.
 int         token_rows(long long rows);
@@ -17,7 +18,7 @@ cudaError_t paged_token_prepare(PagedType type, PagedType cache, int head_dim); 
 cudaError_t paged_token_launch(const AttendParams& p, PagedType type, PagedType cache, int head_dim, int rows, int used_rows,
                                cudaStream_t stream);
 
-// Prompts; max_new: the most new tokens of a sequence, sms: of the device. No workspace.
+// Prompts; max_new: the most new tokens of a sequence. No workspace.
 cudaError_t paged_prompt_prepare(PagedType type, PagedType cache, int head_dim);
 cudaError_t paged_prompt_launch(const AttendParams& p, PagedType type, PagedType cache, int head_dim, int max_new, int sms, cudaStream_t stream);
 

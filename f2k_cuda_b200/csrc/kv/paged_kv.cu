@@ -173,6 +173,15 @@ int f2k_kv_create(const f2k_kv_config* cfg, f2k_kv** out) {
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, h->device);
     if (e != cudaSuccess) return fail_cuda(h, "cudaDeviceGetAttribute", e);
     if (major != 10) return fail(h, F2K_ERR_UNSUPPORTED, "this library contains sm_100a code only (needs a B200-class GPU)");
+    // The pages are read and written for as long as the handle lives: they have to be where its kernels run.
+    for (const void* x : {(const void*)c.k_pages, (const void*)c.v_pages, (const void*)c.k_scale, (const void*)c.v_scale}) {
+        cudaPointerAttributes a{};
+        if (x == nullptr) continue;
+        e = cudaPointerGetAttributes(&a, x);
+        if (e != cudaSuccess) return fail_cuda(h, "cudaPointerGetAttributes", e);
+        if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != h->device))
+            return fail(h, F2K_ERR_INVALID, "pages and scales must lie in the current device's memory");
+    }
     e = paged_token_prepare((PagedType)c.type, (PagedType)c.cache_type, c.head_dim);
     if (e == cudaSuccess) e = paged_prompt_prepare((PagedType)c.type, (PagedType)c.cache_type, c.head_dim);
     if (e != cudaSuccess) return fail_cuda(h, "kernel load", e);
@@ -202,31 +211,31 @@ void f2k_kv_destroy(f2k_kv* h) {
 
 const char* f2k_kv_last_error(const f2k_kv* h) { return h ? h->err.c_str() : "no handle"; }
 
-int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const void* q, const void* k, const void* v, const void* gamma_q,
-                  const void* gamma_k, const float* cos_table, const float* sin_table, int n_positions, float eps, void* q_out,
-                  const f2k_kv_strides* strides, void* stream) {
+int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const f2k_kv_append_args* args, void* stream) {
     if (const int rc = check_ready(h)) return rc;
     const f2k_kv_config& c = h->cfg;
     AppendParams p{};
     if (const int rc = check_batch(h, batch, p.batch)) return rc;
+    if (!args) return fail(h, F2K_ERR_INVALID, "null arguments");
+    const f2k_kv_append_args& a = *args;
     if (p.batch.n_seqs == 0) return F2K_OK;
-    if (!q || !k || !v || !q_out) return fail(h, F2K_ERR_INVALID, "null tensor pointer");
-    if (!gamma_q != !gamma_k) return fail(h, F2K_ERR_INVALID, "one gain without the other");
-    if (c.rot_dim > 0 && (!cos_table || !sin_table || n_positions <= 0)) return fail(h, F2K_ERR_INVALID, "null rotation table");
-    for (const void* x : {q, k, v, (const void*)q_out, gamma_q, gamma_k, (const void*)cos_table, (const void*)sin_table})
+    if (!a.q || !a.k || !a.v || !a.q_out) return fail(h, F2K_ERR_INVALID, "null tensor pointer");
+    if (!a.gamma_q != !a.gamma_k) return fail(h, F2K_ERR_INVALID, "one gain without the other");
+    if (c.rot_dim > 0 && (!a.cos_table || !a.sin_table || a.n_positions <= 0)) return fail(h, F2K_ERR_INVALID, "null rotation table");
+    const void* pointers[8] = {a.q, a.k, a.v, a.q_out, a.gamma_q, a.gamma_k, a.cos_table, a.sin_table};
+    for (const void* x : pointers)
         if (misaligned(x, 16)) return fail(h, F2K_ERR_INVALID, "tensors, gains and tables must be 16-byte aligned");
-    const f2k_kv_strides none{}, &st = strides ? *strides : none;
-    if (const int rc = take_stride(h, st.q, c.n_heads, "q", p.q_stride)) return rc;
-    if (const int rc = take_stride(h, st.k, c.n_kv_heads, "k", p.k_stride)) return rc;
-    if (const int rc = take_stride(h, st.v, c.n_kv_heads, "v", p.v_stride)) return rc;
-    if (const int rc = take_stride(h, st.q_out, c.n_heads, "q_out", p.qo_stride)) return rc;
-    p.q = q, p.k = k, p.v = v, p.gamma_q = gamma_q, p.gamma_k = gamma_k, p.cos_tab = cos_table, p.sin_tab = sin_table;
-    p.k_scale = c.k_scale, p.v_scale = c.v_scale, p.q_out = q_out, p.k_pages = c.k_pages, p.v_pages = c.v_pages;
+    if (const int rc = take_stride(h, a.q_stride, c.n_heads, "q", p.q_stride)) return rc;
+    if (const int rc = take_stride(h, a.k_stride, c.n_kv_heads, "k", p.k_stride)) return rc;
+    if (const int rc = take_stride(h, a.v_stride, c.n_kv_heads, "v", p.v_stride)) return rc;
+    if (const int rc = take_stride(h, a.q_out_stride, c.n_heads, "q_out", p.qo_stride)) return rc;
+    p.q = a.q, p.k = a.k, p.v = a.v, p.gamma_q = a.gamma_q, p.gamma_k = a.gamma_k, p.cos_tab = a.cos_table, p.sin_tab = a.sin_table;
+    p.k_scale = c.k_scale, p.v_scale = c.v_scale, p.q_out = a.q_out, p.k_pages = c.k_pages, p.v_pages = c.v_pages;
     p.kp_page = c.k_page_stride, p.kp_head = c.k_head_stride, p.kp_tok = c.k_token_stride;
     p.vp_page = c.v_page_stride, p.vp_head = c.v_head_stride, p.vp_tok = c.v_token_stride;
     p.n_heads = c.n_heads, p.n_kv_heads = c.n_kv_heads, p.page_shift = h->page_shift, p.n_pages = c.n_pages;
-    p.n_positions = n_positions, p.rot_dim = c.rot_dim, p.interleaved = c.interleaved, p.eps = eps, p.status = h->d_status;
-    const cudaError_t e = kv_append_launch(p, (PagedType)c.type, (PagedType)c.cache_type, c.head_dim, static_cast<cudaStream_t>(stream));
+    p.n_positions = a.n_positions, p.rot_dim = c.rot_dim, p.interleaved = c.interleaved, p.eps = a.eps, p.status = h->d_status;
+    const cudaError_t e = kv_append_launch(p, (PagedType)c.type, (PagedType)c.cache_type, c.head_dim, h->sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? F2K_OK : fail_cuda(h, "append launch", e);
 }
 
@@ -235,19 +244,20 @@ size_t f2k_kv_workspace_bytes(const f2k_kv* h, const f2k_kv_batch* batch) {
     return workspace_of(h, rows_of(h, batch)).bytes;
 }
 
-int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const void* q, void* o, float* lse, const f2k_kv_strides* strides,
-                  void* workspace, size_t workspace_bytes, void* stream) {
+int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const f2k_kv_attend_args* args, void* stream) {
     if (const int rc = check_ready(h)) return rc;
     const f2k_kv_config& c = h->cfg;
     AttendParams p{};
     if (const int rc = check_batch(h, batch, p.batch)) return rc;
+    if (!args) return fail(h, F2K_ERR_INVALID, "null arguments");
+    const f2k_kv_attend_args& a = *args;
     if (p.batch.n_seqs == 0) return F2K_OK;
-    if (!q || !o) return fail(h, F2K_ERR_INVALID, "null tensor pointer");
-    if (misaligned(q, 16) || misaligned(o, 16) || misaligned(lse, 4)) return fail(h, F2K_ERR_INVALID, "q and o must be 16-byte aligned");
-    const f2k_kv_strides none{}, &st = strides ? *strides : none;
-    if (const int rc = take_stride(h, st.q, c.n_heads, "q", p.q_stride)) return rc;
-    if (const int rc = take_stride(h, st.o, c.n_heads, "o", p.o_stride)) return rc;
-    p.q = q, p.o = o, p.lse = lse, p.k_scale = c.k_scale, p.v_scale = c.v_scale;
+    if (!a.q || !a.o) return fail(h, F2K_ERR_INVALID, "null tensor pointer");
+    if (misaligned(a.q, 16) || misaligned(a.o, 16)) return fail(h, F2K_ERR_INVALID, "q and o must be 16-byte aligned");
+    if (misaligned(a.lse, 4)) return fail(h, F2K_ERR_INVALID, "lse must be 4-byte aligned");
+    if (const int rc = take_stride(h, a.q_stride, c.n_heads, "q", p.q_stride)) return rc;
+    if (const int rc = take_stride(h, a.o_stride, c.n_heads, "o", p.o_stride)) return rc;
+    p.q = a.q, p.o = a.o, p.lse = a.lse, p.k_scale = c.k_scale, p.v_scale = c.v_scale;
     p.n_heads = c.n_heads, p.n_kv_heads = c.n_kv_heads, p.group = group_of(h), p.page_shift = h->page_shift, p.n_pages = c.n_pages;
     p.window = c.window, p.scale_log2 = h->scale * 1.4426950408889634f, p.status = h->d_status;
     p.wait_limit_clk = h->wait_clk > 0 ? h->wait_clk : kDefaultWaitClk;
@@ -260,15 +270,15 @@ int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const void* q, void* o, 
     }
     const int rows = rows_of(h, batch);
     const Workspace ws = workspace_of(h, rows);
-    if (!workspace || workspace_bytes < ws.bytes) return fail(h, F2K_ERR_WORKSPACE, "workspace smaller than f2k_kv_workspace_bytes");
-    if (misaligned(workspace, 16)) return fail(h, F2K_ERR_INVALID, "workspace must be 16-byte aligned");
+    if (!a.workspace || a.workspace_bytes < ws.bytes) return fail(h, F2K_ERR_WORKSPACE, "workspace smaller than f2k_kv_workspace_bytes");
+    if (misaligned(a.workspace, 16)) return fail(h, F2K_ERR_INVALID, "workspace must be 16-byte aligned");
     // The kernel counts units in 32 bits.
     const int unit = token_unit_keys(c.head_dim * (c.cache_type == F2K_E4M3 ? 1 : 2));
     const long long keys = (long long)batch->table_width << h->page_shift;
     const double tiles = (double)batch->n_tokens * p.group / rows + batch->n_seqs;
     if (tiles * c.n_kv_heads * (double)(keys / unit + 1 + kWorkCost) >= 4294967295.0)
         return fail(h, F2K_ERR_UNSUPPORTED, "the batch could hold 2^32 pieces of work: make two calls of it");
-    uint8_t* w = static_cast<uint8_t*>(workspace);
+    uint8_t* w = static_cast<uint8_t*>(a.workspace);
     p.ws_join = reinterpret_cast<JoinJob*>(w + ws.join);
     p.ws_ml = reinterpret_cast<float2*>(w + ws.ml);
     p.ws_o = reinterpret_cast<float*>(w + ws.o);

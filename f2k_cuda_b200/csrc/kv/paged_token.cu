@@ -122,7 +122,7 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
         if (w < warp) upto += ctl.scan[w];
         total += ctl.scan[w];
     }
-    const int n_pieces = pieces(total, p.n_ctas, kWorkCost + KW);
+    const int n_pieces = pieces(total, p.n_ctas, kLeastPlaces);
     const int cta = blockIdx.x;
     if (cta >= n_pieces || total == 0) {
         if (threadIdx.x == 0) p.ws_join[cta].n = 0;

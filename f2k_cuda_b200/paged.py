@@ -12,19 +12,26 @@ the wrong type, shape or device raises TypeError.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import KvBatch, KvConfig, KvStrides, lib
+from ._lib import KvBatch, KvConfig, lib
 from ._stream import stream_handle
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 
 
+# struct f2k_kv_append_args, f2k_kv_attend_args: written whole by one call. (As 14 arguments of the C function, each
+# converted by ctypes, they cost the host 2 us more.)
+_APPEND = struct.Struct("8Q4qif")
+_ATTEND = struct.Struct("3Q2q2Q")
+
+
 def _p(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 class PagedBatch:
@@ -43,7 +50,7 @@ class PagedBatch:
         if cu_seqlens is None and max_new != 1:
             raise TypeError("without cu_seqlens every sequence has one new token")
         self.kv_lens, self.page_table, self.cu_seqlens, self.max_new = kv_lens, page_table, cu_seqlens, max_new
-        self.device = kv_lens.device
+        self.index = kv_lens.get_device()
         self._c = KvBatch(n, 0, max_new, page_table.shape[1], page_table.stride(0) if n > 1 else 0, _p(cu_seqlens), _p(kv_lens),
                           _p(page_table))
         self._ref = C.byref(self._c)
@@ -85,7 +92,10 @@ class PagedKV:
                                   or t.device != k_pages.device):
                 raise TypeError("scales must be contiguous float32 [n_kv_heads] on the pages' device")
         self.k_pages, self.v_pages, self.k_scale, self.v_scale = k_pages, v_pages, k_scale, v_scale
-        self.device = k_pages.device
+        self.device, self._index = k_pages.device, k_pages.get_device()
+        self._args = bytearray(max(_APPEND.size, _ATTEND.size))       # a handle is used from one thread at a time
+        self._args_at = C.addressof(C.c_char.from_buffer(self._args))
+        self._dtype, self._heads, self._kv_heads, self._dim, self._half = cfg.dtype, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.rot_dim // 2
         c = KvConfig(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.page_size, cfg.n_pages, _TYPES[cfg.dtype],
                      _TYPES[k_pages.dtype], cfg.rot_dim, int(cfg.interleaved), cfg.window, cfg.scale, _p(k_pages), _p(v_pages),
                      *k_pages.stride()[:3], *v_pages.stride()[:3], _p(k_scale), _p(v_scale))
@@ -114,49 +124,66 @@ class PagedKV:
     def workspace_size_bytes(self, batch: PagedBatch) -> int:
         return int(lib.f2k_kv_workspace_bytes(self._h, batch._ref)) if self.ok() else 0
 
+    # The checks are most of what a call of a few tokens costs the host (8 appended tokens 9.9 us a call when every tensor's
+    # strides and device object were looked at), so the plain case asks little.
     def _stride(self, t, rows, heads):
-        """Token stride of a [rows, heads, head_dim] tensor of the layer."""
+        """Token stride of a [rows, heads, head_dim] tensor of the layer; 0: dense."""
+        if t.dtype is not self._dtype or t.get_device() != self._index:
+            raise TypeError(f"expected {self._dtype} on {self.device}")
+        if t.is_contiguous() and t.numel() == rows * heads * self._dim:
+            return 0
         s = t.stride()
-        if t.dtype is not self.cfg.dtype or t.shape != (rows, heads, self.cfg.head_dim) or s[2] != 1 \
-                or (heads > 1 and s[1] != self.cfg.head_dim) or t.device != self.device:
-            raise TypeError(f"expected {self.cfg.dtype} [{rows}, {heads}, {self.cfg.head_dim}] on {self.device}, heads dense")
+        if t.shape != (rows, heads, self._dim) or s[2] != 1 or (heads > 1 and s[1] != self._dim):
+            raise TypeError(f"expected [{rows}, {heads}, {self._dim}], a token's heads dense")
         return s[0] if rows > 1 else 0
+
+    def _vector(self, t, dtype, numel, what):
+        if t.dtype is not dtype or t.get_device() != self._index or t.numel() != numel or not t.is_contiguous():
+            raise TypeError(f"{what} must be contiguous {dtype} with {numel} elements on {self.device}")
+        return t.data_ptr()
 
     def append(self, Q, K, V, gammas, tables, eps, Q_out, batch: PagedBatch, stream=None) -> bool:
         """K and V of the batch's new tokens into the cache, Q to Q_out (which may be Q), both normalised and rotated on the
         way. gammas = (gamma_q, gamma_k), [head_dim] of Config.dtype, or (None, None); tables = (cos, sin), fp32
         [positions, rot_dim / 2], or (None, None) with rot_dim 0."""
-        if not self.ok():
+        if self._rc:
             return False
-        c, n = self.cfg, Q.shape[0]
-        st = KvStrides(self._stride(Q, n, c.n_heads), self._stride(K, n, c.n_kv_heads), self._stride(V, n, c.n_kv_heads),
-                       self._stride(Q_out, n, c.n_heads), 0)
-        for g in gammas:
-            if g is not None and (g.dtype is not c.dtype or g.shape != (c.head_dim,) or not g.is_contiguous() or g.device != self.device):
-                raise TypeError("gains must be contiguous [head_dim] of the layer's type")
+        n, stride = Q.shape[0], self._stride
+        gamma_q, gamma_k = gammas
         cos, sin = tables
         positions = 0
-        if cos is not None and sin is not None:
+        if cos is not None and self._half:
             positions = cos.shape[0]
-            for t in (cos, sin):
-                if t.dtype is not torch.float32 or t.shape != (positions, c.rot_dim // 2) or not t.is_contiguous() or t.device != self.device:
-                    raise TypeError("tables must be contiguous float32 [positions, rot_dim / 2]")
-        if batch.device != self.device:
+            cos = self._vector(cos, torch.float32, positions * self._half, "tables")
+        if sin is not None and self._half:
+            sin = self._vector(sin, torch.float32, positions * self._half, "tables")
+        if gamma_q is not None:
+            gamma_q = self._vector(gamma_q, self._dtype, self._dim, "gains")
+        if gamma_k is not None:
+            gamma_k = self._vector(gamma_k, self._dtype, self._dim, "gains")
+        if batch.index != self._index:
             raise TypeError("the batch lies on another device than the cache")
-        return lib.f2k_kv_append(self._h, batch._with(n), _p(Q), _p(K), _p(V), _p(gammas[0]), _p(gammas[1]), _p(cos), _p(sin),
-                                 positions, eps, _p(Q_out), C.byref(st), stream_handle(stream)) == _lib.F2K_OK
+        _APPEND.pack_into(self._args, 0, Q.data_ptr(), K.data_ptr(), V.data_ptr(), gamma_q or 0, gamma_k or 0,
+                          cos if self._half and cos else 0, sin if self._half and sin else 0, Q_out.data_ptr(),
+                          stride(Q, n, self._heads), stride(K, n, self._kv_heads), stride(V, n, self._kv_heads), stride(Q_out, n, self._heads),
+                          positions, eps)
+        return lib.f2k_kv_append(self._h, batch._with(n), self._args_at, stream_handle(stream)) == _lib.F2K_OK
 
     def attend(self, Q, O, batch: PagedBatch, workspace, lse=None, stream=None) -> bool:
         """O = softmax(scale Q K^T) V of the batch's new tokens over the keys that they see; lse: fp32 [tokens, n_heads],
         the logarithm of the softmax's sum. O may be Q."""
-        if not self.ok():
+        if self._rc:
             return False
-        c, n = self.cfg, Q.shape[0]
-        st = KvStrides(self._stride(Q, n, c.n_heads), 0, 0, 0, self._stride(O, n, c.n_heads))
-        if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (n, c.n_heads) or not lse.is_contiguous()
-                                or lse.device != self.device):
-            raise TypeError("lse must be contiguous float32 [tokens, n_heads]")
-        if batch.device != self.device or (workspace is not None and (workspace.device != self.device or not workspace.is_contiguous())):
-            raise TypeError("batch and workspace must lie on the cache's device")
-        return lib.f2k_kv_attend(self._h, batch._with(n), _p(Q), _p(O), _p(lse), C.byref(st), _p(workspace),
-                                 0 if workspace is None else workspace.nbytes, stream_handle(stream)) == _lib.F2K_OK
+        n = Q.shape[0]
+        q, o = self._stride(Q, n, self._heads), self._stride(O, n, self._heads)
+        if lse is not None:
+            lse = self._vector(lse, torch.float32, n * self._heads, "lse")
+        if batch.index != self._index:
+            raise TypeError("the batch lies on another device than the cache")
+        size = 0
+        if workspace is not None:
+            size = workspace.nbytes
+            if size and (workspace.get_device() != self._index or not workspace.is_contiguous()):
+                raise TypeError("the workspace must be contiguous and on the cache's device")
+        _ATTEND.pack_into(self._args, 0, Q.data_ptr(), O.data_ptr(), lse or 0, q, o, _p(workspace), size)
+        return lib.f2k_kv_attend(self._h, batch._with(n), self._args_at, stream_handle(stream)) == _lib.F2K_OK

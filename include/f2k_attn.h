@@ -432,34 +432,47 @@ typedef struct f2k_kv_batch {
     const int32_t* page_table;
 } f2k_kv_batch;
 
-/* Token strides in elements (multiples of 8, heads dense); 0 = dense. k and v: n_kv_heads heads. */
-typedef struct f2k_kv_strides {
-    long long q, k, v, q_out, o;
-} f2k_kv_strides;
+/* What f2k_kv_append takes beside the batch. q, q_out: [n_tokens][n_heads][head_dim], k, v: [n_tokens][n_kv_heads]
+ * [head_dim]; q_out may be q. gamma_q, gamma_k: [head_dim] gains of a per-head RMSNorm in front of the rotation, or both
+ * NULL for none. cos_table, sin_table: fp32 [n_positions][rot_dim / 2], row = position; not read with rot_dim 0.
+ * Strides between token rows in elements (multiples of 8, a token's heads dense); 0 = dense. */
+typedef struct f2k_kv_append_args {
+    const void *q, *k, *v, *gamma_q, *gamma_k;
+    const float *cos_table, *sin_table;
+    void* q_out;
+    long long q_stride, k_stride, v_stride, q_out_stride;
+    int   n_positions;
+    float eps;
+} f2k_kv_append_args;
+
+/* What f2k_kv_attend takes beside the batch: q, o [n_tokens][n_heads][head_dim] (o may be q), lse fp32
+ * [n_tokens][n_heads] or NULL, token strides as above, and its workspace. */
+typedef struct f2k_kv_attend_args {
+    const void* q;
+    void*  o;
+    float* lse;
+    long long q_stride, o_stride;
+    void*  workspace;
+    size_t workspace_bytes;
+} f2k_kv_attend_args;
 
 /* *out is set whenever memory for a handle could be had, so that the message can be read. */
 int         f2k_kv_create(const f2k_kv_config* cfg, f2k_kv** out);
 void        f2k_kv_destroy(f2k_kv* h);
 const char* f2k_kv_last_error(const f2k_kv* h);
 
-/* q_out = rotated (normalised) q; k likewise and v go to the cache. q, q_out: [n_tokens][n_heads][head_dim],
- * k, v: [n_tokens][n_kv_heads][head_dim]; q_out may be q. gamma_q, gamma_k: [head_dim] gains of a per-head
- * RMSNorm in front of the rotation, or both NULL for none. cos, sin: fp32 [n_positions][rot_dim / 2], row =
- * position; NULL with rot_dim 0. fp32 arithmetic, one rounding. */
-int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const void* q, const void* k, const void* v,
-                  const void* gamma_q, const void* gamma_k, const float* cos_table, const float* sin_table,
-                  int n_positions, float eps, void* q_out, const f2k_kv_strides* strides, void* stream);
+/* q_out = rotated (normalised) q; k likewise, and v, go to the cache. fp32 arithmetic, one rounding. */
+int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const f2k_kv_append_args* args, void* stream);
 
 /* Bytes of workspace that f2k_kv_attend needs for a batch of this n_seqs and max_new (0 for prompts).
  * Calls whose GPU work may overlap need one each. */
 size_t f2k_kv_workspace_bytes(const f2k_kv* h, const f2k_kv_batch* batch);
 
 /* o = softmax(scale q K^T) V over the keys that each token sees; zero for a token that sees none.
- * lse: fp32 [n_tokens][n_heads], the logarithm of the sum of exp(scale q K^T) (-inf for none), or
- * NULL. Tokens of a call do not see values of later tokens, but a value that is not finite can make
- * the outputs of up to 255 tokens before it NaN; what lies in pages beyond kv_lens does not matter. */
-int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const void* q, void* o, float* lse,
-                  const f2k_kv_strides* strides, void* workspace, size_t workspace_bytes, void* stream);
+ * lse: the logarithm of the sum of exp(scale q K^T), -inf for none. Tokens of a call do not see values
+ * of later tokens, but a value that is not finite can make the outputs of up to 255 tokens before it NaN;
+ * what lies in pages beyond kv_lens does not matter. */
+int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const f2k_kv_attend_args* args, void* stream);
 
 /* Reads and clears the status word of this handle's kernels (0 = clean); synchronises the handle's
  * device. F2K_ERR_DEVICE and a message when it is not zero. */

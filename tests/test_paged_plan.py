@@ -53,7 +53,7 @@ static void one(std::mt19937& r, bool wild) {
     }
     start.push_back(total);
     if (total == 0) return;
-    const int n_pieces = pieces(total, n_ctas, kWorkCost + KW);
+    const int n_pieces = pieces(total, n_ctas, kLeastPlaces);
     CHECK(piece_begin(total, n_pieces, 0) == 0 && piece_begin(total, n_pieces, n_pieces) == total);
     using Id = std::tuple<int, int, int>;                       // sequence, head, row tile
     std::map<Id, std::set<int>> keys;                           // units taken
