@@ -21,7 +21,7 @@
 //    waits for such a tile and clears them before it hands the tile over. That is the last tile, or the first ones of a
 //    window. K and V have a ring and a loader each: K of the tile after next may come in as soon as S is done with its slot.
 //  * Q is fetched by the softmax groups themselves (the rows of a tile are a gather once group is not a power of two).
-//  * Scores are masked by key number, only in tiles that some row of the warp does not see whole.
+//  * Scores are masked by key number, in tensor memory, only in tiles that some row of the warp does not see whole.
 //
 // e4m3 caches: a tile comes in as bytes into the second half of its slot, and its loader turns it into fp16 (exactly) in place,
 // row by row, before it hands it over; rows of V to be cleared are written as zeros then. The products are fp16 ones; bf16
@@ -52,7 +52,6 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColP0 = 128, kColP1 = 192, kColO0 = 256, kColO1 = 384;
 constexpr float kLazyThreshold = 8.0f;                  // log2 units
 constexpr int kPParts = 2;
-constexpr int kBoxRing = 16;                            // tiles whose page flags are kept; the loader is at most six ahead
 
 constexpr int kMostStages = 4;
 template <int D>
@@ -72,7 +71,7 @@ struct Ctl {
     uint64_t clean;                                     // a V tile that has to be cleared in part has arrived
     uint32_t tmem_base;
     uint32_t abort;
-    uint32_t boxes[kBoxRing];                           // pages of a key tile that were fetched, a bit each
+    int2 see[2][kRows];                                 // [group][row]: keys that the row sees
     float row_scale[2][kRows];                          // e4m3 with bf16 queries: what a row of S is multiplied by
 };
 
@@ -215,7 +214,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     if (*reinterpret_cast<volatile uint32_t*>(&ctl->tmem_base) != tmem) ctl->abort = 1;
 
     if (warp >= 8) {
-        setmaxnreg_dec<88>();
+        setmaxnreg_dec<56>();
         if (warp == kLoadK || warp == kLoadV) {
             // ------------------------------ loaders: a lane per page and piece ------------------------------
             const int kv = warp == kLoadK ? 0 : 1;
@@ -295,7 +294,6 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 const uint32_t bar = kE4m3 ? smem_u32(&ctl->raw[kv][slot]) : clear ? smem_u32(&ctl->clean) : full;
                 const uint32_t dst = smem + kSmemRing + (kv * kSlots + slot) * kTileBytes, in = dst + (kE4m3 ? kTileBytes / 2 : 0);
                 if (lane == 0) {
-                    if (kv == 0) ctl->boxes[j % kBoxRing] = boxes;
                     mbar_arrive_expect_tx(bar, (uint32_t)__popc(boxes) * (kE4m3 ? 1 : kPieces) * (uint32_t)box_rows * kRowBytes);
                 }
                 __syncwarp();
@@ -440,7 +438,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         }
     } else if (any) {
         // ------------------------------ softmax groups ------------------------------
-        setmaxnreg_inc<208>();
+        setmaxnreg_inc<224>();
         const int t = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + kColS, tP = tmem + lane_base + (t == 0 ? kColP0 : kColP1);
@@ -493,8 +491,58 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             if (lane == 0) mbar_arrive(smem_u32(&ctl->q_full[t]));
         }
         const int r = (warp & 3) * 32 + lane;
-        KeyRange see{0, 0x7fffffff};                    // of this thread's row; rows that do not exist are not masked
-        if (r < rows) see = visible_keys(job.s, tok0 + token_of(r), p.window);
+        // Steps [clean0, clean1) have nothing to mask in this warp. What a row sees is kept in shared memory: the other steps read
+        // it there, and these need its registers (rows that do not exist see everything and end nowhere).
+        int clean0, clean1;
+        {
+            KeyRange see{0, 0x7fffffff};
+            if (r < rows) see = visible_keys(job.s, tok0 + token_of(r), p.window);
+            ctl->see[t][r] = make_int2(see.lo, see.hi);
+            const int lo_max = __reduce_max_sync(0xffffffffu, see.lo), hi_min = __reduce_min_sync(0xffffffffu, see.hi);
+            const int first = max(0, (lo_max - key00 + kKeys - 1) / kKeys), end = hi_min <= key00 ? 0 : min(n_kv, (hi_min - key00) / kKeys);
+            clean0 = pair ? first : (first + 1 - t) >> 1;
+            clean1 = pair ? end : (end + 1 - t) >> 1;
+        }
+        // The other steps' scores are masked where they lie, in tensor memory, chunk by chunk of 32 keys and only the chunks that
+        // are cut, in front of the step proper: with the masks inside it, behind a test, every step paid for them in registers
+        // and order of instructions (8192 tokens 499 us, without any masks 443; the step compiled twice, 523 to 540).
+        const int box_shift = min(p.page_shift, 7);
+        auto hide = [&](int tile, uint32_t bad) {
+            const int base = key00 + tile * kKeys;
+            const int2 see = ctl->see[t][(warp & 3) * 32 + lane];
+            const int first = see.x - base, end = see.y - base;
+#pragma unroll 1
+            for (int from = 0; from < kKeys; from += 32) {
+                if (bad == 0u && !__any_sync(0xffffffffu, end < from + 32 || first > from)) continue;
+                uint32_t v[32];
+                tmem_ld_x32(tS + from, v);
+                const bool bad0 = bad >> (from >> box_shift) & 1u, bad1 = bad >> ((from + 16) >> box_shift) & 1u;
+                const int lo0 = bad0 ? from + 16 : first, hi1 = bad1 ? from + 16 : end;      // either half of the chunk may be gone
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (from + k < lo0 || from + k >= end) v[k] = __float_as_uint(-INFINITY);
+#pragma unroll
+                for (int k = 16; k < 32; ++k)
+                    if (from + k < first || from + k >= hi1) v[k] = __float_as_uint(-INFINITY);
+                tmem_st_x32(tS + from, v);
+            }
+            tmem_wait_st();
+        };
+        // Pages outside the cache: whether there are any is looked up once, while the first key tile is on its way, and which
+        // only where there are. (A word in shared memory, written by the loader and read every step, cost 4 to 8 % of the whole,
+        // the MMAs' operands keeping shared memory busy; a step's pages looked up a step ahead by the warp itself, 5 %.)
+        const int32_t* pages = p.batch.table + job.b * p.batch.table_stride;
+        bool strays = false;
+#pragma unroll 4
+        for (int k = (lo >> p.page_shift) + lane; k < (hi + (1 << p.page_shift) - 1) >> p.page_shift; k += 32)
+            strays |= (unsigned)pages[k] >= (unsigned)p.n_pages;
+        strays = __any_sync(0xffffffffu, strays);
+        auto bad_pages = [&](int tile) {
+            const int k = key00 + tile * kKeys + (lane << box_shift);
+            const bool bad = lane < kKeys >> box_shift && k < hi && k + (1 << box_shift) > lo && (unsigned)pages[k >> p.page_shift] >= (unsigned)p.n_pages;
+            return __ballot_sync(0xffffffffu, bad);
+        };
         float m_ref = -INFINITY, l_sum = 0.0f;
         if constexpr (kE4m3 && std::is_same_v<T, __nv_bfloat16>) {
             if (t == 1 && !pair) {                      // the rows are group 0's
@@ -505,33 +553,16 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             }
         }
         bool ok = true;
-        const uint32_t all_boxes = (1u << (kKeys / min(kKeys, 1 << p.page_shift))) - 1u;
-
         const int n = steps(t);
         for (int i = 0; i < n; ++i) {
             ok = mbar_wait(smem_u32(&ctl->s_full[t]), i & 1, abort_flag, wait_limit);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after_sync();
-            const int tile = tile_of(t, i), base = key00 + tile * kKeys;
+            if (i < clean0 || i >= clean1 || strays) hide(tile_of(t, i), strays ? bad_pages(tile_of(t, i)) : 0u);
+
             uint32_t s[128];
             float mx[kMaxChains];
-            uint32_t boxes;
-            bool masked;
-            auto hide = [&](int from) {                 // scores [from, from + 64) of keys that the row does not see
-                const int first = see.lo - base, end = see.hi - base;
-#pragma unroll
-                for (int k = from; k < from + 64; ++k)
-                    if (k < first || k >= end) s[k] = __float_as_uint(-INFINITY);
-                if (boxes != all_boxes) {
-#pragma unroll
-                    for (int k = from; k < from + 64; k += 16)
-                        if (!(boxes >> (k >> min(p.page_shift, 7)) & 1u)) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) s[k + e] = __float_as_uint(-INFINITY);
-                        }
-                }
-            };
             {
                 uint32_t(&s0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[0]);
                 uint32_t(&s1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32]);
@@ -539,19 +570,15 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 uint32_t(&s3)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[96]);
                 tmem_ld_x32(tS + 0, s0);
                 tmem_ld_x32(tS + 32, s1);
-                boxes = *reinterpret_cast<volatile uint32_t*>(&ctl->boxes[tile % kBoxRing]);
-                masked = __any_sync(0xffffffffu, base < see.lo || base + kKeys > see.hi) || boxes != all_boxes;
                 tmem_wait_ld();
                 tmem_ld_x32(tS + 64, s2);
                 tmem_ld_x32(tS + 96, s3);
-                if (masked) hide(0);
                 row_max64<true>(&s[0], mx);
                 tmem_wait_ld();
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&ctl->s_free));
             }
-            if (masked) hide(64);
             row_max64<false>(&s[64], mx);
             const float m_tile = row_max_finish(mx);
             const bool pv_seen = i == 0 || mbar_test(smem_u32(&ctl->pv_done[t]), (i - 1) & 1);
