@@ -53,7 +53,7 @@ __device__ Token look_up(const AppendParams& p, int t) {
         cu0 = b.cu[seq], cu1 = b.cu[seq + 1];
         if (t < cu0 || t >= cu1) return r;            // behind the last sequence
     }
-    const SeqView s = seq_view(cu0, cu1, b.lens[seq], b.n_tokens, (long long)b.table_width << p.page_shift);
+    const SeqView s = seq_view(cu0, cu1, b.lens[seq], b.n_tokens, b.max_new, (long long)b.table_width << p.page_shift);
     const int pos = s.len - s.n_new + (t - s.first);
     if (s.bad || pos < 0) {
         atomicOr(p.status, (int)kStatusBadLength);
@@ -283,6 +283,22 @@ cudaError_t launch(const AppendParams& p, int sms, cudaStream_t stream) {
 }
 
 }  // namespace
+
+cudaError_t kv_append_prepare(PagedType type, PagedType cache, int head_dim, bool interleaved) {
+    cudaFuncAttributes attr;
+    auto load = [&](auto t, auto e, auto d, auto i) {
+        using T = decltype(t);
+        constexpr bool kE = decltype(e)::value, kI = decltype(i)::value;
+        const cudaError_t r = cudaFuncGetAttributes(&attr, kv_append_kernel<T, kE, decltype(d)::value, kI, 1>);
+        return r == cudaSuccess ? cudaFuncGetAttributes(&attr, kv_append_kernel<T, kE, decltype(d)::value, kI, 4>) : r;
+    };
+    auto by_pairs = [&](auto t, auto e, auto d) { return interleaved ? load(t, e, d, std::true_type{}) : load(t, e, d, std::false_type{}); };
+    auto by_dim = [&](auto t, auto e) {
+        return head_dim == 64 ? by_pairs(t, e, std::integral_constant<int, 64>{}) : by_pairs(t, e, std::integral_constant<int, 128>{});
+    };
+    auto by_cache = [&](auto t) { return cache == kE4m3 ? by_dim(t, std::true_type{}) : by_dim(t, std::false_type{}); };
+    return type == kBf16 ? by_cache(__nv_bfloat16{}) : by_cache(__half{});
+}
 
 cudaError_t kv_append_launch(const AppendParams& p, PagedType type, PagedType cache, int head_dim, int sms, cudaStream_t stream) {
     auto by_dim = [&](auto t, auto e) {

@@ -7,13 +7,15 @@
 
 namespace f2k {
 
+// *_prepare: load the kernels on the current device, so that the first call can be a captured one.
+cudaError_t kv_append_prepare(PagedType type, PagedType cache, int head_dim, bool interleaved);
 // sms: of the device, here and below.
 cudaError_t kv_append_launch(const AppendParams& p, PagedType type, PagedType cache, int head_dim, int sms, cudaStream_t stream);
 
 // Query rows of a work that the token kernel's variants hold: 8, 16, 32 or 64; and the CTAs it runs with.
 int         token_rows(long long rows);
 int         token_ctas(int sms);
-cudaError_t paged_token_prepare(PagedType type, PagedType cache, int head_dim);   // load the kernels on the current device
+cudaError_t paged_token_prepare(PagedType type, PagedType cache, int head_dim);
 // rows: of a tile, one of token_rows(); used_rows: the most that any tile of the call has.
 cudaError_t paged_token_launch(const AttendParams& p, PagedType type, PagedType cache, int head_dim, int rows, int used_rows,
                                cudaStream_t stream);

@@ -75,7 +75,7 @@ int check_batch(f2k_kv* h, const f2k_kv_batch* b, PagedBatch& out) {
     if (misaligned(b->kv_lens, 4) || misaligned(b->page_table, 4) || misaligned(b->cu_seqlens, 4))
         return fail(h, F2K_ERR_INVALID, "lengths and page table must be 4-byte aligned");
     if (!b->cu_seqlens && b->n_tokens < b->n_seqs) return fail(h, F2K_ERR_INVALID, "fewer tokens than sequences without cu_seqlens");
-    out = PagedBatch{b->cu_seqlens, b->kv_lens, b->page_table, stride, b->table_width, b->n_seqs, b->n_tokens};
+    out = PagedBatch{b->cu_seqlens, b->kv_lens, b->page_table, stride, b->table_width, b->n_seqs, b->n_tokens, b->max_new};
     return F2K_OK;
 }
 
@@ -183,6 +183,7 @@ int f2k_kv_create(const f2k_kv_config* cfg, f2k_kv** out) {
             return fail(h, F2K_ERR_INVALID, "pages and scales must lie in the current device's memory");
     }
     e = paged_token_prepare((PagedType)c.type, (PagedType)c.cache_type, c.head_dim);
+    if (e == cudaSuccess) e = kv_append_prepare((PagedType)c.type, (PagedType)c.cache_type, c.head_dim, c.interleaved != 0);
     if (e == cudaSuccess) e = paged_prompt_prepare((PagedType)c.type, (PagedType)c.cache_type, c.head_dim);
     if (e != cudaSuccess) return fail_cuda(h, "kernel load", e);
     const int unit = token_unit_keys(c.head_dim * (c.cache_type == F2K_E4M3 ? 1 : 2));

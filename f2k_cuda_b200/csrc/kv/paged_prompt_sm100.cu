@@ -114,7 +114,7 @@ __device__ __forceinline__ bool find_job(const AttendParams& p, int tokens_per_t
     for (int b0 = 0; b0 < b.n_seqs; b0 += 32) {
         const int i = b0 + lane;
         SeqView s{0, 0, 0, false};
-        if (i < b.n_seqs) s = seq_view(b.cu ? b.cu[i] : i, b.cu ? b.cu[i + 1] : i + 1, b.lens[i], b.n_tokens, (long long)b.table_width << p.page_shift);
+        if (i < b.n_seqs) s = seq_view(b.cu ? b.cu[i] : i, b.cu ? b.cu[i + 1] : i + 1, b.lens[i], b.n_tokens, b.max_new, (long long)b.table_width << p.page_shift);
         if (s.bad && lane == i - b0) atomicOr(p.status, (int)kStatusBadLength);
         const int tiles = (s.n_new + tokens_per_tile - 1) / tokens_per_tile, ctas = (tiles + per_cta - 1) / per_cta;
         int upto = ctas;
@@ -767,6 +767,7 @@ cudaError_t paged_prompt_launch(const AttendParams& p, PagedType type, PagedType
         return (by_tokens < by_most ? by_tokens : by_most) * p.n_kv_heads;
     };
     const int per_cta = ctas(2) >= sms ? 2 : 1;
+    if (ctas(per_cta) > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;

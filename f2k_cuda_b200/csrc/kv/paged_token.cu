@@ -63,7 +63,7 @@ struct Ctl {
     uint64_t full[kMostStages], empty[kMostStages];
     uint32_t boxes[kMostStages];               // which boxes of the stage hold keys
     float2 ml[kWarps][32];
-    unsigned scan[kWarps];
+    unsigned long long scan[kWarps];
     unsigned seq_begin;
     int seq;
     uint32_t abort;
@@ -101,27 +101,29 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
     };
     const int per = (p.batch.n_seqs + kThreads - 1) / kThreads;
     const int b_first = min(p.batch.n_seqs, (int)threadIdx.x * per), b_last = min(p.batch.n_seqs, b_first + per);
-    unsigned mine = 0;
+    unsigned long long mine = 0;                              // 64 bits: rows of malformed batches may overlap and add up to anything
     for (int b = b_first; b < b_last; ++b) {
         const SeqView s = seq_of(p.batch, p.page_shift, b);
         if (s.bad) atomicOr(p.status, (int)kStatusBadLength);
         if (held) ctl.first[b] = s.first, ctl.n_new[b] = s.n_new, ctl.len[b] = s.len;
         mine += seq_places(p, seq_work(s, p.group, S::kRows, kUnit, p.window));
     }
-    unsigned upto = mine;
+    unsigned long long upto = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const unsigned v = __shfl_up_sync(0xffffffffu, upto, d);
+        const unsigned long long v = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += v;
     }
     if (lane == 31) ctl.scan[warp] = upto;
     __syncthreads();
-    unsigned total = 0;
+    unsigned long long all_places = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
         if (w < warp) upto += ctl.scan[w];
-        total += ctl.scan[w];
+        all_places += ctl.scan[w];
     }
+    const unsigned total = all_places >> 32 ? 0u : (unsigned)all_places;
+    if (all_places >> 32 && threadIdx.x == 0) atomicOr(p.status, (int)kStatusBadLength);
     const int n_pieces = pieces(total, p.n_ctas, kLeastPlaces);
     const int cta = blockIdx.x;
     if (cta >= n_pieces || total == 0) {
@@ -130,7 +132,7 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
     }
     const unsigned begin = piece_begin(total, n_pieces, cta), end = piece_begin(total, n_pieces, cta + 1);
     if (begin >= upto - mine && begin < upto) {
-        unsigned at = upto - mine;
+        unsigned at = (unsigned)(upto - mine);
         for (int b = b_first;; ++b) {
             const unsigned places = seq_places(p, seq_work(seq(b), p.group, S::kRows, kUnit, p.window));
             if (begin - at < places) {

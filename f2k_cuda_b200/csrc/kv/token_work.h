@@ -18,7 +18,7 @@ constexpr unsigned kWorkCost = 8;
 constexpr int kLeastPlaces = 8;
 
 F2K_HD SeqView seq_of(const PagedBatch& b, int page_shift, int i) {
-    return seq_view(b.cu ? b.cu[i] : i, b.cu ? b.cu[i + 1] : i + 1, b.lens[i], b.n_tokens, (long long)b.table_width << page_shift);
+    return seq_view(b.cu ? b.cu[i] : i, b.cu ? b.cu[i + 1] : i + 1, b.lens[i], b.n_tokens, b.max_new, (long long)b.table_width << page_shift);
 }
 F2K_HD unsigned seq_places(const AttendParams& p, const SeqWork& w) {
     return (unsigned)w.row_tiles * ((unsigned)w.n_units + kWorkCost) * (unsigned)p.n_kv_heads;

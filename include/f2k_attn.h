@@ -418,13 +418,13 @@ typedef struct f2k_kv_config {
  * them is at position kv_lens[b] - 1. Rows behind the last sequence are left as they are. Key j lies
  * in page page_table[b * table_stride + j / page_size]. Sequences may share pages that nobody appends
  * to; a page that receives tokens belongs to one sequence.
- * Lengths that do not fit (negative, longer than the table's row, shorter than the new tokens, rows
- * outside the call's) and page numbers outside the cache never make a kernel reach outside: such
+ * Lengths that do not fit (negative, longer than the table's row, shorter than the new tokens, more of
+ * those than max_new, rows outside the call's) and page numbers outside the cache never make a kernel reach outside: such
  * tokens are not appended, such keys not attended, and f2k_kv_device_status reports it. */
 typedef struct f2k_kv_batch {
     int n_seqs;
     int n_tokens;               /* rows of the call's tensors */
-    int max_new;                /* the most new tokens that a sequence has: decides which kernel attends */
+    int max_new;                /* at least the new tokens of any sequence: decides which kernel attends */
     int table_width;            /* pages in a row of the table */
     long long table_stride;     /* int32 between rows; 0: table_width */
     const int32_t* cu_seqlens;  /* [n_seqs + 1]; NULL: one new token per sequence, row b for sequence b */

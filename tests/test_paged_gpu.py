@@ -193,6 +193,9 @@ def test_bad_pages_and_lengths_are_reported():
         p.cu.copy_(torch.tensor(cu, dtype=torch.int32))
         p.attend()
         assert p.kv.device_status() & 32
+    p.cu.copy_(torch.tensor([0, 2, 3, 3], dtype=torch.int32))           # two new tokens where max_new says one
+    p.attend()
+    assert p.kv.device_status() == 32
     p.cu.copy_(torch.arange(4, dtype=torch.int32))
     p.attend()
     p.check_attend()
@@ -336,6 +339,69 @@ def test_captured_and_replayed_with_other_lengths():
         graph.replay()
         p.check_attend()
     assert p.kv.device_status() == 0
+
+
+@pytest.fixture(scope="module")
+def late_copy(tmp_path_factory):
+    """late_copy(dst, src): a copy that lets its successor start at once and writes some 0.3 ms later."""
+    import ctypes as C
+    import subprocess
+    from pathlib import Path
+
+    from f2k_cuda_b200.build import NVCC_FLAGS, _nvcc
+    so = tmp_path_factory.mktemp("late") / "late_copy.so"
+    subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", str(Path(__file__).parent / "cpp" / "late_copy.cu"), "-o", str(so)], check=True)
+    lib = C.CDLL(str(so))
+    lib.late_copy.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p]
+
+    def copy(dst, src):
+        assert dst.is_contiguous() and src.is_contiguous() and dst.nbytes == src.nbytes and dst.nbytes % 16 == 0
+        assert lib.late_copy(dst.data_ptr(), src.data_ptr(), dst.nbytes, 600_000, torch.cuda.current_stream().cuda_stream) == 0
+    return copy
+
+
+@pytest.mark.parametrize("late", ["q", "lens_t", "cu", "table", "k_pages", "v_pages"])
+@pytest.mark.parametrize("news,lens", [([1] * 4, [300, 20, 64, 1000]), ([200, 1, 40, 60], [300, 20, 64, 1000])], ids=["tokens", "prompts"])
+def test_attend_behind_a_late_writer(late_copy, late, news, lens):
+    """Every input may be written by the kernel in front while this one's blocks already stand ready."""
+    p = Problem(news + [0] * 3, lens + [0] * 3, 8, 2, 128, 16, BF, seed=30)        # 7 sequences: 8 offsets; lengths padded below
+    import f2k_cuda_b200 as f2k
+    room = torch.zeros(8, dtype=torch.int32, device="cuda")
+    room[:7] = p.lens_t
+    table = torch.zeros(8, p.table.shape[1], dtype=torch.int32, device="cuda")
+    table[:7] = p.table
+    tensors = {"q": p.q, "lens_t": room, "cu": p.cu, "table": table, "k_pages": p.k_pages, "v_pages": p.v_pages}
+    batch = f2k.PagedBatch(room[:7], table[:7], p.cu, max(news))
+    right = tensors[late].clone()
+    wrong = torch.zeros_like(right)
+    tensors[late].copy_(wrong)
+    torch.cuda.synchronize()
+    late_copy(tensors[late], right)
+    assert p.kv.attend(p.q, p.o, batch, p.ws, lse=p.lse)
+    p.check_attend()
+    assert p.kv.device_status() == 0
+
+
+@pytest.mark.parametrize("late", ["q", "k", "lens_t", "table", "cos", "gain"])
+def test_append_behind_a_late_writer(late_copy, late):
+    import f2k_cuda_b200 as f2k
+    p = Problem([70, 1, 33, 8], [70, 9, 100, 8], 8, 2, 128, 16, BF, rot=128, seed=31)
+    cos, sin = torch.rand(128, 64, device="cuda"), torch.rand(128, 64, device="cuda")
+    gain = torch.rand(128, device="cuda").to(BF)
+    expect = [torch.empty_like(p.q), torch.empty_like(p.q)]
+    tensors = {"q": p.q, "k": p.k, "lens_t": p.lens_t, "table": p.table, "cos": cos, "gain": gain}
+    caches = []
+    for i in range(2):
+        p.k_pages.fill_(3.0)
+        right = tensors[late].clone()
+        if i:
+            tensors[late].zero_()
+            torch.cuda.synchronize()
+            late_copy(tensors[late], right)
+        assert p.kv.append(p.q, p.k, p.v, (gain, gain), (cos, sin), 1e-6, expect[i], p.batch)
+        caches.append(p.k_pages.clone())
+    assert p.kv.device_status() == 0
+    assert torch.equal(expect[0], expect[1]) and torch.equal(caches[0], caches[1])
 
 
 def test_two_streams_with_a_workspace_each():

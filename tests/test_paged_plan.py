@@ -41,7 +41,7 @@ static void one(std::mt19937& r, bool wild) {
     }
     const int n_tokens = cu.back() + pick(0, 3);
     if (wild) for (auto* v : {&cu, &lens}) for (auto& x : *v) if (!pick(0, 2)) x = (int)(r() - (1u << 31)) >> pick(0, 30);
-    p.batch = PagedBatch{cu.data(), lens.data(), nullptr, width, width, n, n_tokens};
+    p.batch = PagedBatch{cu.data(), lens.data(), nullptr, width, width, n, n_tokens, 60};
     const int n_ctas = pick(1, 12);
 
     auto seq = [&](int b) { return seq_of(p.batch, p.page_shift, b); };

@@ -52,6 +52,7 @@ cudaError_t cudaGetDriverEntryPoint(const char*, void** fn, unsigned long long, 
 static int launched_kernel = 0, launched_rows = 0;       // 1 append, 2 token, 3 prompt
 static int* last_status;
 namespace f2k {
+cudaError_t kv_append_prepare(PagedType, PagedType, int, bool) { return cudaSuccess; }
 cudaError_t kv_append_launch(const AppendParams& p, PagedType, PagedType, int, int, cudaStream_t) { ++work; launched_kernel = 1; last_status = p.status; return cudaSuccess; }
 int token_rows(long long rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 int token_ctas(int sms) { return 2 * sms; }
