@@ -12,8 +12,10 @@
 //           half the time: 1024 tokens behind 15001, 16 heads of 64, 154 us.)
 //
 // Roles as in the joint-attention kernel (attn_fwd_sm100.cu): warps 0-3 / 4-7 the softmax groups (one thread per row),
-// warps 8 and 10 the loaders of K and V, warp 9 the tcgen05 issuer, one S buffer in tensor memory that the groups use in turn, P
-// from tensor memory, lazily moved reference maxima. What differs:
+// warps 8 and 10 the loaders of K and V, warp 9 the tcgen05 issuer, P from tensor memory, lazily moved reference maxima. With
+// head_dim 128 tensor memory has one S buffer, which the groups use in turn; with 64 each has its own (Columns), and is then
+// bound by its own softmax: some 2000 clk a step, of which 1024 are the special-function unit's; with one buffer a group
+// waited another 900 to 1200 for its S. What differs from that kernel:
 //
 //  * A loader brings a key tile in page by page: a lane per page and 128-byte piece of head_dim looks its page up (a
 //    tile ahead) and issues its own TMA box. Rows of V that no query of the CTA may see - the rest of the last page,
@@ -49,17 +51,25 @@ constexpr int kThreads = 384, kLoadK = 8, kMmaWarp = 9, kLoadV = 10;
 constexpr int kRows = 128, kKeys = kPromptTile;
 constexpr uint32_t kPieceBytes = 128 * 128;             // 128 rows of 128 bytes
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColS = 0, kColP0 = 128, kColP1 = 192, kColO0 = 256, kColO1 = 384;
 constexpr float kLazyThreshold = 8.0f;                  // log2 units
 constexpr int kPParts = 2;
 
 constexpr int kMostStages = 4;
+// Tensor memory: S and O in fp32, P two values a column.
+template <int D>
+struct Columns {
+    static constexpr bool kOwnS = D == 64;
+    static __host__ __device__ constexpr uint32_t s(int t) { return kOwnS ? 128 * t : 0; }
+    static __host__ __device__ constexpr uint32_t p(int t) { return (kOwnS ? 256 : 128) + 64 * t; }
+    static __host__ __device__ constexpr uint32_t o(int t) { return (kOwnS ? 384 : 256) + D * t; }
+};
+
 template <int D>
 constexpr int kStages = D == 64 ? 4 : 2;                // tiles of K, and of V, in flight or in use: 64 KB each
 
 struct Ctl {
     uint64_t q_full[2];
-    uint64_t s_free;
+    uint64_t s_free[2];                                 // S is in registers; one buffer: [0]
     uint64_t p_full[2][kPParts];
     uint64_t joined;                                    // split form: group 1 has left its share (these: four arrivals each)
     uint64_t full[2][kMostStages];                      // [K, V][slot]
@@ -164,6 +174,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     constexpr int kPieces = D / 64;                     // 128-byte pieces of a row
     constexpr uint32_t kTileBytes = kPieces * kPieceBytes;
     constexpr int kSlots = kStages<D>;
+    constexpr bool kOwnS = Columns<D>::kOwnS;
     constexpr uint32_t kQBytes = kQArea<D>, kSmemQ = 0, kSmemRing = 2 * kQBytes;      // K slots, then V slots
     using M = std::conditional_t<kE4m3, __half, T>;     // the type of the products
     constexpr uint32_t kFormat = std::is_same_v<M, __nv_bfloat16> ? 1u : 0u;
@@ -340,7 +351,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             const uint64_t q0_desc = umma_smem_desc(smem + kSmemQ, 16, 1024), q1_desc = umma_smem_desc(smem + kSmemQ + (pair ? kQBytes : 0), 16, 1024);
             const uint64_t k_desc0 = umma_smem_desc(smem + kSmemRing, 16, 1024);
             const uint64_t v_desc0 = umma_smem_desc(smem + kSmemRing + kSlots * kTileBytes, kPieceBytes, 1024);
-            const uint32_t bar_full0 = smem_u32(&ctl->full[0][0]), bar_empty0 = smem_u32(&ctl->empty[0][0]), bar_free = smem_u32(&ctl->s_free);
+            const uint32_t bar_full0 = smem_u32(&ctl->full[0][0]), bar_empty0 = smem_u32(&ctl->empty[0][0]), bar_free = smem_u32(&ctl->s_free[0]);
             // Every wait is looked at ahead, in front of the MMAs before it; a look at a barrier that the warp has seen complete
             // before (the second group's at a tile of a pair) costs nothing more.
             auto slot_off16 = [&](int j) { return (uint32_t)(j % kSlots) * (kTileBytes >> 4); };
@@ -351,17 +362,20 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             auto par_full = [&](int j) { return (uint32_t)(j / kSlots) & 1u; };
             auto release = [&](int kv, int j) { umma_commit(bar_empty0 + (kv * kMostStages + j % kSlots) * 8); };
             auto bar_p = [&](int t, int part) { return smem_u32(&ctl->p_full[t][part]); };
-            // The order is S0_0, then S1_i, P1 V_(i-1), S0_(i+1), P0 V_i: S0_i is use 2i of the S buffer and S1_i use 2i + 1, and a use
-            // waits for the release of the one before. The two forms are compiled apart: this warp's instructions are what a tile
+            // With one S buffer the order is S0_0, then S1_i, P1 V_(i-1), S0_(i+1), P0 V_i: S0_i is use 2i of the buffer and S1_i use
+            // 2i + 1, and a use waits for the release of the one before. The two forms are compiled apart: this warp's instructions are what a tile
             // costs (with `pair` looked at as it goes the pair form took 6 % longer).
             auto run = [&](auto form) {
                 constexpr bool kPair = decltype(form)::value;
                 auto tile = [](int t, int i) { return kPair ? i : 2 * i + t; };
                 const int n0 = kPair ? n_kv : (n_kv + 1) >> 1, n1 = kPair ? n_kv : n_kv >> 1;
+                // S_t of step i: K's tile (seen before where the other group of a pair had it), and the S buffer read: its own, step
+                // i - 1; or the one that both use.
                 auto look_s = [&](int t, int i) {
                     const int j = tile(t, i);
-                    if (kPair && t == 1) return peek(bar_free, 0u);                    // K_i is there
-                    return peek(bar_full(0, j), par_full(j), bar_free, t == 1 ? 0u : 1u);
+                    const uint32_t free = bar_free + (kOwnS ? t * 8 : 0), par = kOwnS ? (uint32_t)(i - 1) & 1u : t == 1 ? 0u : 1u;
+                    if (kPair && t == 1) return peek(free, par);
+                    return peek(bar_full(0, j), par_full(j), free, par);
                 };
                 auto look_p = [&](int t, int i) {
                     const int j = tile(t, i);
@@ -372,15 +386,16 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                     tc_fence_after_sync();
                     const int j = tile(t, i);
                     const uint64_t q = t == 0 ? q0_desc : q1_desc, k = k_desc0 + slot_off16(j);
-                    if constexpr (kPieces == 2) umma_ss_x8(tmem + kColS, q, k, idesc_s);
-                    else umma_ss_x4(tmem + kColS, q, k, idesc_s);
+                    const uint32_t d = tmem + (t == 0 ? Columns<D>::s(0) : Columns<D>::s(1));
+                    if constexpr (kPieces == 2) umma_ss_x8(d, q, k, idesc_s);
+                    else umma_ss_x4(d, q, k, idesc_s);
                     umma_commit(smem_u32(&ctl->s_full[t]));
                     if (t == 1 || !kPair) release(0, j);
                 };
                 // O_t (+)= P_t V_j, half by half as the softmax group hands P over; `next` takes the look at what follows.
                 auto issue_pv = [&](int t, int i, const Look& first, auto&& next) -> bool {
                     const int j = tile(t, i);
-                    const uint32_t d = tmem + (t == 0 ? kColO0 : kColO1), a = tmem + (t == 0 ? kColP0 : kColP1);
+                    const uint32_t d = tmem + (t == 0 ? Columns<D>::o(0) : Columns<D>::o(1)), a = tmem + (t == 0 ? Columns<D>::p(0) : Columns<D>::p(1));
                     const uint64_t v = v_desc0 + slot_off16(j);
                     if (!finish(first)) return false;
                     const Look half = peek(bar_p(t, 1), (uint32_t)i & 1u);
@@ -399,8 +414,36 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                     ok = bars.wait(smem_u32(&ctl->q_full[0]), 0) && bars.wait(bar_full(0, 0), 0);
                     if (ok) issue_s(0, 0);
                     if (ok && kPair) ok = bars.wait(smem_u32(&ctl->q_full[1]), 0);
-                    if (n1 > 0) s_look = look_s(1, 0);
                 }
+                if constexpr (kOwnS) {
+                    // S0_0, S1_0, then S0_(i+1), P0 V_i, S1_(i+1), P1 V_i.
+                    if (ok && n1 > 0) {
+                        if (!kPair) ok = bars.wait(bar_full(0, tile(1, 0)), par_full(tile(1, 0)));
+                        if (ok) issue_s(1, 0);
+                    }
+                    if (n0 > 1) s_look = look_s(0, 1);
+                    for (int i = 0; i < n0 && ok; ++i) {
+                        if (i + 1 < n0) {
+                            if (!(ok = finish(s_look))) break;
+                            p_look = look_p(0, i);
+                            issue_s(0, i + 1);
+                        } else {
+                            p_look = look_p(0, i);
+                        }
+                        if (!(ok = issue_pv(0, i, p_look, [&] { if (i + 1 < n1) s_look = look_s(1, i + 1); }))) break;
+                        if (i >= n1) break;
+                        if (i + 1 < n1) {
+                            if (!(ok = finish(s_look))) break;
+                            p_look = look_p(1, i);
+                            issue_s(1, i + 1);
+                        } else {
+                            p_look = look_p(1, i);
+                        }
+                        if (!(ok = issue_pv(1, i, p_look, [&] { if (i + 2 < n0) s_look = look_s(0, i + 2); }))) break;
+                    }
+                    return;
+                }
+                if (n1 > 0) s_look = look_s(1, 0);
                 for (int i = 0; i < n0 && ok; ++i) {
                     if (i < n1) {
                         if (!(ok = finish(s_look))) break;
@@ -441,8 +484,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         setmaxnreg_inc<224>();
         const int t = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t tS = tmem + lane_base + kColS, tP = tmem + lane_base + (t == 0 ? kColP0 : kColP1);
-        const uint32_t tO = tmem + lane_base + (t == 0 ? kColO0 : kColO1);
+        const uint32_t tS = tmem + lane_base + Columns<D>::s(t), tP = tmem + lane_base + Columns<D>::p(t), tO = tmem + lane_base + Columns<D>::o(t);
         float c = p.scale_log2;                         // of this thread's row
         if (kE4m3 && p.k_scale != nullptr) c *= p.k_scale[kvh];
         const int tok0 = (job.tile0 + (pair ? t : 0)) * per_tile, rows = min(per_tile, job.s.n_new - tok0) * p.group;
@@ -577,7 +619,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 tmem_wait_ld();
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl->s_free));
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->s_free[kOwnS ? t : 0]));
             }
             row_max64<false>(&s[64], mx);
             const float m_tile = row_max_finish(mx);
