@@ -34,6 +34,12 @@ def _p(t):
     return 0 if t is None else t.data_ptr()
 
 
+def _strides(pages):
+    """Page, head and token stride; of a dimension of one element, whose stride says nothing, that of a dense array."""
+    dense = pages.shape[1] * pages.shape[2] * pages.shape[3], pages.shape[2] * pages.shape[3], pages.shape[3]
+    return [s if n > 1 else d for n, s, d in zip(pages.shape, pages.stride(), dense)]
+
+
 class PagedBatch:
     """The sequences of a call. kv_lens int32 [n]: lengths with the new tokens. page_table int32 [n, width], rows may be
     strided. cu_seqlens int32 [n + 1]: rows of the new tokens; None: one each. max_new: the most new tokens that a
@@ -45,6 +51,8 @@ class PagedBatch:
             if t is not None and (t.dtype is not torch.int32 or t.dim() != dims or (t.shape[-1] > 1 and t.stride(-1) != 1)
                                   or t.device != kv_lens.device):
                 raise TypeError("lengths and page table must be int32 on one device, rows contiguous")
+        if n > 1 and page_table.stride(0) < page_table.shape[1]:      # an expanded row: 0 would mean dense
+            raise TypeError("the rows of page_table must not overlap")
         if page_table.shape[0] != n or (cu_seqlens is not None and cu_seqlens.shape[0] != n + 1):
             raise TypeError("kv_lens [n], page_table [n, width] and cu_seqlens [n + 1] belong together")
         if cu_seqlens is None and max_new != 1:
@@ -87,6 +95,8 @@ class PagedKV:
             if tuple(t.shape) != shape or t.dtype not in _TYPES or t.dtype != k_pages.dtype or t.device != k_pages.device \
                     or t.stride(3) != 1:
                 raise TypeError(f"pages must be {list(shape)}, both of one type and device, rows contiguous")
+            if any(n > 1 and s <= 0 for n, s in zip(shape, t.stride())):
+                raise TypeError("pages must not be expanded")
         for t in (k_scale, v_scale):
             if t is not None and (t.dtype is not torch.float32 or tuple(t.shape) != (cfg.n_kv_heads,) or not t.is_contiguous()
                                   or t.device != k_pages.device):
@@ -98,7 +108,7 @@ class PagedKV:
         self._dtype, self._heads, self._kv_heads, self._dim, self._half = cfg.dtype, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.rot_dim // 2
         c = KvConfig(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.page_size, cfg.n_pages, _TYPES[cfg.dtype],
                      _TYPES[k_pages.dtype], cfg.rot_dim, int(cfg.interleaved), cfg.window, cfg.scale, _p(k_pages), _p(v_pages),
-                     *k_pages.stride()[:3], *v_pages.stride()[:3], _p(k_scale), _p(v_scale))
+                     *_strides(k_pages), *_strides(v_pages), _p(k_scale), _p(v_scale))
         self._rc = lib.f2k_kv_create(C.byref(c), C.byref(self._h))
 
     def __del__(self):
@@ -133,8 +143,8 @@ class PagedKV:
         if t.is_contiguous() and t.numel() == rows * heads * self._dim:
             return 0
         s = t.stride()
-        if t.shape != (rows, heads, self._dim) or s[2] != 1 or (heads > 1 and s[1] != self._dim):
-            raise TypeError(f"expected [{rows}, {heads}, {self._dim}], a token's heads dense")
+        if t.shape != (rows, heads, self._dim) or s[2] != 1 or (heads > 1 and s[1] != self._dim) or (rows > 1 and s[0] < heads * self._dim):
+            raise TypeError(f"expected [{rows}, {heads}, {self._dim}], a token's heads dense, rows apart")
         return s[0] if rows > 1 else 0
 
     def _vector(self, t, dtype, numel, what):

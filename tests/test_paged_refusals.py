@@ -339,6 +339,37 @@ def test_attend_checks_its_tensors(kv):
     assert not paged.lib.calls
 
 
+def test_expanded_tensors_are_refused(kv):
+    """A stride of 0 means dense to the C functions: an expanded view would be read far behind its memory."""
+    from f2k_cuda_b200 import paged
+    a = _args()
+    for name, heads in (("Q", 4), ("K", 2), ("V", 2), ("Q_out", 4)):
+        with pytest.raises(TypeError):
+            kv.append(**{**a, name: torch.zeros(1, heads, 64, dtype=torch.bfloat16).expand(3, -1, -1)})
+    with pytest.raises(TypeError):
+        kv.append(**{**a, "Q": torch.zeros(600, dtype=torch.bfloat16).as_strided((3, 4, 64), (128, 64, 1))})
+    with pytest.raises(TypeError):
+        kv.attend(torch.zeros(1, 4, 64, dtype=torch.bfloat16).expand(3, -1, -1), a["Q_out"], a["batch"], None)
+    lens = torch.ones(3, dtype=torch.int32)
+    for args in ((lens, torch.zeros(1, 2, dtype=torch.int32).expand(3, -1)), (lens[:1].expand(3), torch.zeros(3, 2, dtype=torch.int32))):
+        with pytest.raises(TypeError):
+            paged.PagedBatch(*args)
+    cfg = paged.PagedKV.Config(4, 2, 64, 16, 6, rot_dim=32)
+    pages = torch.zeros(6, 2, 16, 64, dtype=torch.bfloat16)
+    for view in (pages[:1].expand(6, -1, -1, -1), pages[:, :1].expand(-1, 2, -1, -1), pages[:1, :1, :1].expand(6, 2, 16, -1)):
+        with pytest.raises(TypeError):
+            paged.PagedKV(cfg, view, pages)
+    assert not paged.lib.calls
+
+
+def test_strides_of_single_pages_and_heads():
+    """A dimension of one element may have any stride; the library gets that of a dense array."""
+    from f2k_cuda_b200.paged import _strides
+    one = torch.zeros(4096).as_strided((1, 1, 16, 64), (0, 0, 128, 1))
+    assert _strides(one) == [1024, 1024, 128]
+    assert _strides(torch.zeros(3, 16, 2, 64).transpose(1, 2)) == [2048, 64, 128]
+
+
 def test_batches_and_caches_check_theirs(kv):
     from f2k_cuda_b200.paged import PagedBatch, PagedKV
     lens, table = torch.ones(3, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32)
