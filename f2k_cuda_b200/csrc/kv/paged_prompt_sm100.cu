@@ -28,7 +28,7 @@
 // e4m3 caches: a tile comes in as bytes into the second half of its slot, and its loader turns it into fp16 (exactly) in place,
 // row by row, before it hands it over; rows of V to be cleared are written as zeros then. The products are fp16 ones; bf16
 // queries are brought into fp16's range by a power of two per row, which goes into the row's exponent factor with the
-// head's scale of K. The token kernel, which converts in registers for every 64 rows anew, took 6.6 ms for 8192 tokens.
+// head's scale of K. (8192 tokens 582 us; 6.6 ms in the token kernel, which converts in registers for every 64 rows anew.)
 //
 // Long tiles first: the grid's first CTAs are the last tiles of every sequence, which see the most keys.
 #include "../attn_params.h"
@@ -53,6 +53,11 @@ constexpr uint32_t kPieceBytes = 128 * 128;             // 128 rows of 128 bytes
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLazyThreshold = 8.0f;                  // log2 units
 constexpr int kPParts = 2;
+// Registers a thread, softmax groups and the other warps, of the 384 * 168 a CTA is launched with; the e4m3 loaders convert.
+template <bool kE4m3>
+constexpr int kRegsSoftmax = kE4m3 ? 216 : 224;
+template <bool kE4m3>
+constexpr int kRegsOther = (384 * 168 - 256 * kRegsSoftmax<kE4m3>) / 128 / 8 * 8;
 
 constexpr int kMostStages = 4;
 // Tensor memory: S and O in fp32, P two values a column.
@@ -225,11 +230,11 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
     if (*reinterpret_cast<volatile uint32_t*>(&ctl->tmem_base) != tmem) ctl->abort = 1;
 
     if (warp >= 8) {
-        setmaxnreg_dec<56>();
+        setmaxnreg_dec<kRegsOther<kE4m3>>();
         if (warp == kLoadK || warp == kLoadV) {
             // ------------------------------ loaders: a lane per page and piece ------------------------------
             const int kv = warp == kLoadK ? 0 : 1;
-            const int box_rows = min(kKeys, 1 << p.page_shift), n_boxes = kKeys / box_rows;
+            const int box_rows = min(kKeys, 1 << p.page_shift), n_boxes = kKeys / box_rows, box_shift = min(p.page_shift, 7);
             const int box = lane & 7, piece = lane >> 3;
             const bool mine = box < n_boxes && piece < (kE4m3 ? 1 : kPieces);
             const uint32_t all_boxes = (1u << n_boxes) - 1u;
@@ -241,37 +246,42 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             };
             auto look_up = [&](int j) { return needed(j) ? row[(key00 + j * kKeys + box * box_rows) >> p.page_shift] : 0; };
             // e4m3: tile j, which has come in, to fp16 where it lies. Rows go up: what row r's 256 (128) bytes of fp16 are written over has
-            // been read before (its own bytes, or rows below it).
+            // been read before (its own bytes, or rows of its batch or below it). Tiles to be cleared in part have a loop of their own
+            // (one loop with a test 732 us for 8192 tokens, apart 605, with eight rows a lane at a time instead of four 582).
             auto convert = [&](int j, uint32_t boxes) -> bool {
                 const int slot = j % kSlots, base = key00 + j * kKeys;
                 if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->raw[kv][slot]), (j / kSlots) & 1, abort_flag, wait_limit))) return false;
                 const bool clear = kv == 1 && (base < lo || base + kKeys > hi || boxes != all_boxes);
                 const uint32_t dst = smem + kSmemRing + (kv * kSlots + slot) * kTileBytes, in = dst + kTileBytes / 2;
-                constexpr int kLanes = D / 16, kAtOnce = 32 / kLanes, kBatch = 4;      // lanes of a row, rows of the warp at once
+                constexpr int kLanes = D / 16, kAtOnce = 32 / kLanes, kBatch = 8;      // lanes of a row, rows of the warp at once
                 const int ch = lane % kLanes;
+                auto rows = [&](auto clears) {
 #pragma unroll 1
-                for (int r0 = lane / kLanes; r0 < kKeys; r0 += kAtOnce * kBatch) {
-                    uint4 v[kBatch];
+                    for (int r0 = lane / kLanes; r0 < kKeys; r0 += kAtOnce * kBatch) {
+                        uint4 v[kBatch];
 #pragma unroll
-                    for (int u = 0; u < kBatch; ++u) {
-                        const int r = r0 + u * kAtOnce, twist = D == 128 ? (r & 7) : ((r >> 1) & 3);
-                        v[u] = ld_shared_v4(in + r * D + ((ch ^ twist) << 4));
-                        if (clear) {
-                            const int key = base + r;
-                            if (!(key >= lo && key < hi && (boxes >> (r / box_rows) & 1u))) v[u] = make_uint4(0, 0, 0, 0);
+                        for (int u = 0; u < kBatch; ++u) {
+                            const int r = r0 + u * kAtOnce, twist = D == 128 ? (r & 7) : ((r >> 1) & 3);
+                            v[u] = ld_shared_v4(in + r * D + ((ch ^ twist) << 4));
+                            if constexpr (decltype(clears)::value) {
+                                const int key = base + r;
+                                if (!(key >= lo && key < hi && (boxes >> (r >> box_shift) & 1u))) v[u] = make_uint4(0, 0, 0, 0);
+                            }
                         }
-                    }
-                    __syncwarp();
+                        __syncwarp();
 #pragma unroll
-                    for (int u = 0; u < kBatch; ++u) {
-                        const int r = r0 + u * kAtOnce;
-                        const Row16 w = f16_of_e4m3x16(v[u]);
-                        const uint32_t at = dst + (ch >> 2) * kPieceBytes + r * 128;
-                        st_shared_v4(at + (((2 * ch & 7) ^ (r & 7)) << 4), w.lo);
-                        st_shared_v4(at + (((2 * ch + 1 & 7) ^ (r & 7)) << 4), w.hi);
+                        for (int u = 0; u < kBatch; ++u) {
+                            const int r = r0 + u * kAtOnce;
+                            const Row16 w = f16_of_e4m3x16(v[u]);
+                            const uint32_t at = dst + (ch >> 2) * kPieceBytes + r * 128;
+                            st_shared_v4(at + (((2 * ch & 7) ^ (r & 7)) << 4), w.lo);
+                            st_shared_v4(at + (((2 * ch + 1 & 7) ^ (r & 7)) << 4), w.hi);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
-                }
+                };
+                if (clear) rows(std::true_type{});
+                else rows(std::false_type{});
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&ctl->full[kv][slot]));
@@ -327,7 +337,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                     ++cleaned;
                     for (int r = lane >> 3; r < kKeys; r += 4) {
                         const int key = base + r;
-                        if (key >= lo && key < hi && (boxes >> (r / box_rows) & 1u)) continue;
+                        if (key >= lo && key < hi && (boxes >> (r >> box_shift) & 1u)) continue;
 #pragma unroll
                         for (int i = 0; i < kPieces; ++i) st_shared_v4(dst + i * kPieceBytes + r * 128 + (lane & 7) * 16, make_uint4(0, 0, 0, 0));
                     }
@@ -481,7 +491,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         }
     } else if (any) {
         // ------------------------------ softmax groups ------------------------------
-        setmaxnreg_inc<224>();
+        setmaxnreg_inc<kRegsSoftmax<kE4m3>>();
         const int t = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + Columns<D>::s(t), tP = tmem + lane_base + Columns<D>::p(t), tO = tmem + lane_base + Columns<D>::o(t);
