@@ -111,13 +111,16 @@ int group_of(const f2k_kv* h) { return h->cfg.n_heads / h->cfg.n_kv_heads; }
 // CTA a sequence and key head then. 16-bit caches, us, token kernel / prompt kernel: 16 sequences of about 27000 keys, 8 key
 // heads, 16 rows 278 / 303, 32 rows 488 / 307, 64 rows 1032 / 323; of 16000 keys, 64 rows: 2 sequences 96 / 133, 4 sequences
 // 171 / 134; 32 rows: 4 sequences 87 / 133, 8 sequences 159 / 135. head_dim 64, 192 CTAs: 32 rows 39 / 41, 64 rows 56 / 41.
-// e4m3, where the prompt kernel is bound by turning bytes into fp16: 32 rows 354 / 707, 64 rows 696 / 708.
+// e4m3, where the prompt kernel is bound by turning bytes into fp16: 32 rows, 16 sequences of about 27000 keys 348 / 555;
+// 36 and 64 rows alike, of 16000 keys: 8 sequences 224 / 279, 10 sequences 275 / 279, 16 sequences 430 / 282; head_dim 64,
+// 8 sequences 126 / 152, of 1000 keys 24 / 17.
 bool takes_prompt_kernel(const f2k_kv* h, const f2k_kv_batch* b) {
     const long long rows = (long long)b->max_new * group_of(h);
     if (b->max_new == 1 || rows <= 16) return false;
     if (rows > 64) return true;
-    if (h->cfg.cache_type == F2K_E4M3 || rows * h->cfg.head_dim <= 2048) return false;
-    return rows * b->n_seqs * h->cfg.n_kv_heads >= 2048;
+    const long long ctas = (long long)b->n_seqs * h->cfg.n_kv_heads;
+    if (h->cfg.cache_type == F2K_E4M3) return rows > 32 && ctas >= 80;
+    return rows * h->cfg.head_dim > 2048 && rows * ctas >= 2048;
 }
 int rows_of(const f2k_kv* h, const f2k_kv_batch* b) { return token_rows((long long)b->max_new * group_of(h)); }
 

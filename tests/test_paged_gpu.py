@@ -47,6 +47,20 @@ def test_several_new_tokens(dtype, cache, dim, window):
     assert p.kv.device_status() == 0
 
 
+@pytest.mark.parametrize("seqs", [39, 40])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [0, 50])
+def test_drafts_over_e4m3_on_both_sides_of_the_rule(seqs, dim, window):
+    """9 to 16 tokens of 4 query heads a key head: below 80 pairs of sequence and key head the token kernel, else the prompts'."""
+    news = [9 + b % 8 for b in range(seqs)]
+    p = Problem(news, [n + 37 * b % 400 for b, n in enumerate(news)], 8, 2, dim, 32, BF, E4, window, scales=True, pad=2, seed=seqs + dim)
+    assert (p.ws.numel() == 0) == (seqs == 40)
+    p.o.fill_(9.0)
+    p.attend()
+    p.check_attend()
+    assert (p.o[-2:] == 9.0).all() and (p.lse[-2:] == 7.0).all() and p.kv.device_status() == 0
+
+
 @pytest.mark.parametrize("cache", [HF, E4], ids=ids)
 @pytest.mark.parametrize("lens", [[20000], [9000, 1], [4097, 12000, 300]])
 def test_long_caches_are_split_and_joined(cache, lens):

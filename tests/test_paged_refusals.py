@@ -204,6 +204,13 @@ int main() {
     if (f2k_kv_device_status(h, &st) != F2K_OK || st != 0) { std::printf("status is not cleared\n"); ++bad; }
     f2k_kv_destroy(h);
     f2k_kv_destroy(nullptr);
+
+    // over an e4m3 cache (2 key heads here) up to 32 rows stay, and so do more rows of fewer than 80 pairs of sequence and key head
+    c = good();
+    c.cache_type = F2K_E4M3;
+    if (f2k_kv_create(&c, &h)) { std::printf("create e4m3\n"); return 1; }
+    takes(8, 100, 2, 32); takes(9, 39, 2, 64); takes(9, 40, 3, 0); takes(16, 39, 2, 64); takes(16, 40, 3, 0); takes(17, 1, 3, 0);
+    f2k_kv_destroy(h);
     return bad;
 }
 """
