@@ -691,8 +691,11 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         }
 
         // ------------------------------ epilogue ------------------------------
-        if (ok && n > 0) {
-            ok = mbar_wait(smem_u32(&ctl->pv_done[t]), (n - 1) & 1, abort_flag, wait_limit);
+        // Rows are parked over the group's Q. The last product stands behind the Q of all four warps; without a step nothing does, and
+        // a warp that is ahead would park its zeros where its neighbour still stores Q.
+        if (ok && (n > 0 || t == 0 || pair)) {
+            ok = n > 0 ? mbar_wait(smem_u32(&ctl->pv_done[t]), (n - 1) & 1, abort_flag, wait_limit)
+                       : mbar_wait(smem_u32(&ctl->q_full[t]), 0, abort_flag, wait_limit);
             ok = __all_sync(0xffffffffu, ok);
         }
         // Split form: group 1 leaves its rows, in fp32, with their references and sums where the key tiles were (once no MMA reads
