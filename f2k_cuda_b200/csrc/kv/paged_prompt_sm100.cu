@@ -288,10 +288,10 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 return true;
             };
             uint32_t came_boxes = 0;                          // e4m3: of the tile that is to be converted next
-            int converted = 0;
-            int next_page = look_up(0), cleaned = 0, j = 0;
+            int converted = 0, issued = 0;                    // issued: tiles whose copies report to `raw` or `full`
+            int next_page = look_up(0), cleaned = 0;
             bool ok = true;
-            for (; j < n_kv; ++j) {
+            for (int j = 0; j < n_kv; ++j) {
                 const int slot = j % kSlots, base = key00 + j * kKeys, page = next_page;
                 next_page = look_up(j + 1);
                 const bool wanted = needed(j), good = wanted && (unsigned)page < (unsigned)p.n_pages;
@@ -322,6 +322,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                     const int first = (base + box * box_rows) & ((1 << p.page_shift) - 1);
                     tma_load_5d(in + piece * kPieceBytes + box * box_rows * kRowBytes, map, bar, 0, first, piece, kvh, page);
                 }
+                if (bar != smem_u32(&ctl->clean)) issued = j + 1;
                 if constexpr (kE4m3) {
                     if (converted < j) {
                         if (!(ok = convert(converted, came_boxes))) break;
@@ -335,6 +336,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     ++cleaned;
+                    issued = j + 1;
                     for (int r = lane >> 3; r < kKeys; r += 4) {
                         const int key = base + r;
                         if (key >= lo && key < hi && (boxes >> (r >> box_shift) & 1u)) continue;
@@ -348,10 +350,10 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
             }
             if (kE4m3 && ok && converted < n_kv) ok = convert(converted, came_boxes);
             if (!ok) {
-                // Leaving early: let the copies this warp started land first (bounded).
+                // Leaving early: let the copies this warp started land first (bounded), the present tile's among them.
                 volatile uint32_t never = 0;
                 if (kv == 1 && !kE4m3) mbar_wait(smem_u32(&ctl->clean), cleaned & 1, &never, 4000000ll);
-                for (int i = max(0, j - kSlots); i < j; ++i)
+                for (int i = max(0, issued - kSlots); i < issued; ++i)
                     mbar_wait(smem_u32(kE4m3 ? &ctl->raw[kv][i % kSlots] : &ctl->full[kv][i % kSlots]), (i / kSlots) & 1, &never, 40000000ll);
             }
         } else if (warp == kMmaWarp) {
