@@ -22,7 +22,7 @@ namespace f2k {
 // Bits of a cache handle's status word, beside kStatusWaitExpired.
 enum PagedStatus : int {
     kStatusBadPage   = 16,   // a page number outside the cache: its tokens are not written, its keys not attended
-    kStatusBadLength = 32,   // a length that the page table cannot hold or below the number of new tokens, or more of those than max_new
+    kStatusBadLength = 32,   // a length that the page table cannot hold or below the number of new tokens; rows outside the call's, or more than max_new
     kStatusBadPosition = 64, // a position behind the rotation tables: the token is not written
 };
 
@@ -35,18 +35,20 @@ struct PagedBatch {
     int n_seqs, n_tokens, max_new;
 };
 
-// New tokens of sequence b, first token, and keys, kept inside what the call can hold whatever the device memory says.
+// New tokens of sequence b, first token, and keys, kept inside what the call can hold whatever the device memory says. A sequence
+// whose rows do not fit has none: the grids are sized by max_new and n_tokens, so a few rows of it would take the places of the
+// sequences behind it, and a part of its rows would stand at positions that are not theirs.
 struct SeqView {
     int first, n_new, len;
     bool bad;
 };
 F2K_HD SeqView seq_view(int cu0, int cu1, int len, int n_tokens, int max_new, long long capacity) {
     SeqView s;
-    s.bad = cu0 < 0 || cu1 < cu0 || cu1 > n_tokens || len < cu1 - cu0 || cu1 - cu0 > max_new || len > capacity;
-    s.first = cu0 < 0 ? 0 : (cu0 > n_tokens ? n_tokens : cu0);
-    const int end = cu1 < s.first ? s.first : (cu1 > n_tokens ? n_tokens : cu1);
-    s.n_new = end - s.first;
+    const bool fits = cu0 >= 0 && cu1 >= cu0 && cu1 <= n_tokens && cu1 - cu0 <= max_new;
+    s.first = fits ? cu0 : 0;
+    s.n_new = fits ? cu1 - cu0 : 0;
     s.len = len < 0 ? 0 : (len > capacity ? (int)capacity : len);
+    s.bad = !fits || len < s.n_new || len > capacity;
     return s;
 }
 

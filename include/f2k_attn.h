@@ -418,9 +418,12 @@ typedef struct f2k_kv_config {
  * them is at position kv_lens[b] - 1. Rows behind the last sequence are left as they are. Key j lies
  * in page page_table[b * table_stride + j / page_size]. Sequences may share pages that nobody appends
  * to; a page that receives tokens belongs to one sequence.
- * Lengths that do not fit (negative, longer than the table's row, shorter than the new tokens, more of
- * those than max_new, rows outside the call's) and page numbers outside the cache never make a kernel reach outside: such
- * tokens are not appended, such keys not attended, and f2k_kv_device_status reports it. */
+ * Lengths and page numbers that do not fit never make a kernel reach outside; f2k_kv_device_status reports them. A sequence
+ * with rows outside the call's, or with more than max_new, has none of them appended or attended: they are left as
+ * they are. Of one with another bad length (negative, longer than the table's row, shorter than its new tokens) nothing is
+ * appended, and its rows are attended with a length of 0 or the row's where it is outside: zero for those that see no key.
+ * Tokens whose page is outside the cache are not appended, keys there not attended. Offsets have to ascend: behind
+ * the first that does not, any sequence may be left out. */
 typedef struct f2k_kv_batch {
     int n_seqs;
     int n_tokens;               /* rows of the call's tensors */

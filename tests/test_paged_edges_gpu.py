@@ -44,3 +44,53 @@ def test_short_wait_limits(dtype, cache, dim, news, lens):
         assert status in (0, 1) if limit else status == 0
         if status == 0:
             p.check_attend()
+
+
+def _call(p, max_new=None, rows=None):
+    """Append and attend with another max_new, or the first `rows` rows of the tensors only; outputs filled with 9."""
+    import f2k_cuda_b200 as f2k
+    p.batch = f2k.PagedBatch(p.lens_t, p.table, p.cu, max_new or max(p.news))
+    p.ws = torch.empty(p.kv.workspace_size_bytes(p.batch), dtype=torch.uint8, device="cuda").fill_(0xAA)
+    n = rows or p.T
+    p.o.fill_(9.0)
+    p.lse.fill_(9.0)
+    assert p.kv.attend(p.q[:n], p.o[:n], p.batch, p.ws, lse=p.lse[:n]), p.kv.last_error()
+    assert p.kv.device_status() == 32
+
+
+# sequence 1 or 0 has more new tokens than max_new says; the rule picks the kernel by max_new
+TOO_MANY = [([1000, 100, 100], 0, 100), ([100, 1000, 100, 7], 1, 100), ([3, 1, 1], 0, 1), ([1, 70, 1], 1, 1), ([4, 30, 3], 1, 4)]
+
+
+@pytest.mark.parametrize("news,wrong,max_new", TOO_MANY, ids=[str(i) for i in range(len(TOO_MANY))])
+@pytest.mark.parametrize("dtype,cache", [(BF, BF), (HF, E4)], ids=ids)
+@pytest.mark.parametrize("behind", [0, 6000])
+def test_a_sequence_with_more_new_tokens_than_max_new(news, wrong, max_new, dtype, cache, behind):
+    """None of its rows is written; the other sequences, those behind it too, are attended as ever."""
+    p = Problem(news, [n + behind for n in news], 8, 2, 128, 16, dtype, cache, seed=sum(news))
+    _call(p, max_new)
+    first = sum(news[:wrong])
+    assert (p.o[first:first + news[wrong]] == 9.0).all() and (p.lse[first:first + news[wrong]] == 9.0).all()
+    p.news[wrong] = 0
+    p.check_attend()
+
+
+@pytest.mark.parametrize("news,rows", [([40, 90, 60], 160), ([1, 2, 1], 3), ([2, 1, 4], 5)], ids=["prompts", "token", "drafts"])
+@pytest.mark.parametrize("dtype,cache", [(BF, BF), (HF, E4)], ids=ids)
+def test_a_sequence_with_rows_behind_the_call_s(news, rows, dtype, cache):
+    """Its first rows lie inside the call's tensors; where they would be in the sequence says the part that does not."""
+    p = Problem(news, [n + 700 for n in news], 8, 2, 64, 16, dtype, cache, seed=sum(news))
+    _call(p, rows=rows)
+    first = sum(news[:2])
+    assert (p.o[first:] == 9.0).all() and (p.lse[first:] == 9.0).all()
+    p.news[2] = 0
+    p.check_attend()
+
+
+def test_a_sequence_with_rows_in_front_of_the_call_s():
+    p = Problem([30, 50, 20], [200, 300, 100], 8, 2, 128, 16, BF, seed=41)
+    p.cu[0] = -8
+    _call(p)
+    assert (p.o[:30] == 9.0).all()
+    p.news[0] = 0
+    p.check_attend()
