@@ -60,4 +60,19 @@ __device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint32_t w) {
     return r;
 }
 
+// What scores over e4m3 keys are multiplied by, never below the smallest normal number: as 0 it would make NaN of a masked score's
+// -inf. Scores of fp16 products are below 2^33, so with a factor this small their weights are all alike.
+__device__ __forceinline__ float score_factor(float scale_log2, const float* k_scale, int head) {
+    const float c = k_scale ? scale_log2 * k_scale[head] : scale_log2;
+    return c < 1.17549435e-38f ? 1.17549435e-38f : c;
+}
+// bf16 queries over e4m3 keys: the exponent field f of the power of two 2^(f - 127) that brings a row's largest element `top` into
+// [2^14, 2^15), for the products in fp16. An infinite one is left as it is, and a row next to nothing is not brought further
+// up than its factor c of the scores can go down by the same power and stay normal: what is lost in front of such a factor has
+// no weight.
+__device__ __forceinline__ unsigned fp16_row_power(float top, float c) {
+    const unsigned e = __float_as_uint(top) >> 23, least = __float_as_uint(c) >> 23;
+    return e == 255u ? 127u : min(min(253u, 268u - e), least + 126u);
+}
+
 }  // namespace f2k

@@ -497,8 +497,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
         const int t = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + Columns<D>::s(t), tP = tmem + lane_base + Columns<D>::p(t), tO = tmem + lane_base + Columns<D>::o(t);
-        float c = p.scale_log2;                         // of this thread's row
-        if (kE4m3 && p.k_scale != nullptr) c *= p.k_scale[kvh];
+        float c = kE4m3 ? score_factor(p.scale_log2, p.k_scale, kvh) : p.scale_log2;        // of this thread's row
         const int tok0 = (job.tile0 + (pair ? t : 0)) * per_tile, rows = min(per_tile, job.s.n_new - tok0) * p.group;
         constexpr int kChunks = D / 8;                  // 16-byte chunks of a row
         const uint32_t q_tile = smem + kSmemQ + (pair ? t : 0) * kQBytes;
@@ -517,7 +516,6 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                 if (r < rows) v[i] = *reinterpret_cast<const uint4*>(q + tok * p.q_stride + (r - tok * p.group) * D);
             }
             if constexpr (kE4m3 && std::is_same_v<T, __nv_bfloat16>) {
-                // the largest element of a row into [2^14, 2^15); an infinite one is left as it is
 #pragma unroll
                 for (int i = 0; i < kChunks; ++i) {
                     using H = Half16<T>;
@@ -527,7 +525,7 @@ paged_prompt_kernel(const __grid_constant__ AttendParams p, const int per_cta) {
                     for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(H::lo(w[k])), fabsf(H::hi(w[k]))));
 #pragma unroll
                     for (int d = 1; d < kChunks; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    const unsigned e = __float_as_uint(top) >> 23, f = e == 255u ? 127u : min(253u, 268u - e);
+                    const unsigned f = fp16_row_power(top, c);
                     const float up = __uint_as_float(f << 23);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) w[k] = Half16<M>::pack(H::lo(w[k]) * up, H::hi(w[k]) * up);

@@ -229,7 +229,7 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
         uint32_t qb[NT][kSteps][2];
         float coef[NT][2];
         KeyRange see[NT][2];
-        const float scale = kE4m3 && p.k_scale ? p.scale_log2 * p.k_scale[x.kvh] : p.scale_log2;
+        const float scale = kE4m3 ? score_factor(p.scale_log2, p.k_scale, x.kvh) : p.scale_log2;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int r = x.rt * S::kRows + rw * 8 * NT + nt * 8 + g8;
@@ -256,9 +256,7 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
                                                fmaxf(fabsf(Half16<T>::lo(raw[ks].y)), fabsf(Half16<T>::hi(raw[ks].y)))));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    // largest element into [2^14, 2^15); an infinite one is left as it is
-                    const unsigned e = __float_as_uint(top) >> 23;
-                    const unsigned f = e == 255u ? 127u : min(253u, 268u - e);
+                    const unsigned f = fp16_row_power(top, scale);
                     const float up = __uint_as_float(f << 23), down = __uint_as_float((254u - f) << 23);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) coef[nt][h] *= __shfl_sync(0xffffffffu, down, (2 * t4 + h) * 4);

@@ -94,3 +94,30 @@ def test_a_sequence_with_rows_in_front_of_the_call_s():
     assert (p.o[:30] == 9.0).all()
     p.news[0] = 0
     p.check_attend()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=ids)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("k_scale", [1.0, 1e-8, 1e-30, 1e-44])
+@pytest.mark.parametrize("news,lens", [([1, 3, 2], [500, 40, 9000]), ([200, 3, 70], [200, 50, 900]), ([600] * 6, [600, 700, 800, 601, 900, 600])],
+                         ids=["tokens", "a tile", "two tiles"])
+def test_rows_of_zeros_over_e4m3(dtype, dim, k_scale, news, lens):
+    """Queries of nothing, or next to nothing: the mean of the values that the row sees, however small the keys' scale is."""
+    p = Problem(news, lens, 16, 4, dim, 32, dtype, E4, window=300, scales=True, seed=dim)
+    p.k_scale.fill_(k_scale)
+    p.q[::2] = 0
+    p.q[1::4, ::3] = 0
+    p.q[1::4, 1::3] *= 1e-38 if dtype is BF else 2.0 ** -20
+    p.attend()
+    p.check_attend()
+    assert p.kv.device_status() == 0
+
+
+def test_small_scales_of_the_scores_over_e4m3():
+    for scale in (1e-20, 1e-38, 1e-45):
+        for news, lens in (([1, 2], [500, 300]), ([100, 300], [200, 300])):
+            p = Problem(news, lens, 8, 2, 128, 16, BF, E4, scales=True, scale=scale, seed=5)
+            p.k_scale.fill_(0.5)
+            p.q[0] = 0
+            p.attend()
+            p.check_attend()
