@@ -12,6 +12,7 @@ the wrong type, shape or device raises TypeError.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import struct
 from dataclasses import dataclass
 
@@ -106,6 +107,7 @@ class PagedKV:
         self._args = bytearray(max(_APPEND.size, _ATTEND.size))       # a handle is used from one thread at a time
         self._args_at = C.addressof(C.c_char.from_buffer(self._args))
         self._dtype, self._heads, self._kv_heads, self._dim, self._half = cfg.dtype, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.rot_dim // 2
+        self._gain = (cfg.head_dim,)
         c = KvConfig(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.page_size, cfg.n_pages, _TYPES[cfg.dtype],
                      _TYPES[k_pages.dtype], cfg.rot_dim, int(cfg.interleaved), cfg.window, cfg.scale, _p(k_pages), _p(v_pages),
                      *_strides(k_pages), *_strides(v_pages), _p(k_scale), _p(v_scale))
@@ -136,20 +138,25 @@ class PagedKV:
 
     # The checks are most of what a call of a few tokens costs the host (8 appended tokens 9.9 us a call when every tensor's
     # strides and device object were looked at), so the plain case asks little.
-    def _stride(self, t, rows, heads):
-        """Token stride of a [rows, heads, head_dim] tensor of the layer; 0: dense."""
+    def _stride(self, t, wanted):
+        """Token stride of a tensor of the layer, `wanted` [rows, heads, head_dim]; 0: dense. A dense one may have its rows in several
+        dimensions, and a token's heads in one."""
         if t.dtype is not self._dtype or t.get_device() != self._index:
             raise TypeError(f"expected {self._dtype} on {self.device}")
-        if t.is_contiguous() and t.numel() == rows * heads * self._dim:
+        shape = t.shape
+        if t.is_contiguous() and (shape == wanted or t.numel() == math.prod(wanted)
+                                  and (shape[-1] == wanted[1] * wanted[2] or shape[-2:] == wanted[1:])):
             return 0
-        s = t.stride()
-        if t.shape != (rows, heads, self._dim) or s[2] != 1 or (heads > 1 and s[1] != self._dim) or (rows > 1 and s[0] < heads * self._dim):
-            raise TypeError(f"expected [{rows}, {heads}, {self._dim}], a token's heads dense, rows apart")
+        s, (rows, heads, dim) = t.stride(), wanted
+        if shape != wanted or s[2] != 1 or (heads > 1 and s[1] != dim) or (rows > 1 and s[0] < heads * dim):
+            raise TypeError(f"expected {list(wanted)}, a token's heads dense, rows apart")
         return s[0] if rows > 1 else 0
 
-    def _vector(self, t, dtype, numel, what):
-        if t.dtype is not dtype or t.get_device() != self._index or t.numel() != numel or not t.is_contiguous():
-            raise TypeError(f"{what} must be contiguous {dtype} with {numel} elements on {self.device}")
+    def _vector(self, t, dtype, shape, what):
+        """Address of a dense tensor of this shape, or of another with as many elements whose rows, if it has any, are as long."""
+        if t.dtype is not dtype or t.get_device() != self._index or not t.is_contiguous() \
+                or (t.shape != shape and (t.numel() != math.prod(shape) or (t.dim() > 1 and t.shape[-1] != shape[-1]))):
+            raise TypeError(f"{what} must be contiguous {dtype} {list(shape)} on {self.device}")
         return t.data_ptr()
 
     def append(self, Q, K, V, gammas, tables, eps, Q_out, batch: PagedBatch, stream=None) -> bool:
@@ -159,23 +166,25 @@ class PagedKV:
         if self._rc:
             return False
         n, stride = Q.shape[0], self._stride
+        q_shape, kv_shape = (n, self._heads, self._dim), (n, self._kv_heads, self._dim)
         gamma_q, gamma_k = gammas
         cos, sin = tables
-        positions = 0
+        positions, table = 0, (0, self._half)
         if cos is not None and self._half:
             positions = cos.shape[0]
-            cos = self._vector(cos, torch.float32, positions * self._half, "tables")
+            table = positions, self._half
+            cos = self._vector(cos, torch.float32, table, "tables")
         if sin is not None and self._half:
-            sin = self._vector(sin, torch.float32, positions * self._half, "tables")
+            sin = self._vector(sin, torch.float32, table, "tables")
         if gamma_q is not None:
-            gamma_q = self._vector(gamma_q, self._dtype, self._dim, "gains")
+            gamma_q = self._vector(gamma_q, self._dtype, self._gain, "gains")
         if gamma_k is not None:
-            gamma_k = self._vector(gamma_k, self._dtype, self._dim, "gains")
+            gamma_k = self._vector(gamma_k, self._dtype, self._gain, "gains")
         if batch.index != self._index:
             raise TypeError("the batch lies on another device than the cache")
         _APPEND.pack_into(self._args, 0, Q.data_ptr(), K.data_ptr(), V.data_ptr(), gamma_q or 0, gamma_k or 0,
                           cos if self._half and cos else 0, sin if self._half and sin else 0, Q_out.data_ptr(),
-                          stride(Q, n, self._heads), stride(K, n, self._kv_heads), stride(V, n, self._kv_heads), stride(Q_out, n, self._heads),
+                          stride(Q, q_shape), stride(K, kv_shape), stride(V, kv_shape), stride(Q_out, q_shape),
                           positions, eps)
         return lib.f2k_kv_append(self._h, batch._with(n), self._args_at, stream_handle(stream)) == _lib.F2K_OK
 
@@ -185,9 +194,10 @@ class PagedKV:
         if self._rc:
             return False
         n = Q.shape[0]
-        q, o = self._stride(Q, n, self._heads), self._stride(O, n, self._heads)
+        shape = n, self._heads, self._dim
+        q, o = self._stride(Q, shape), self._stride(O, shape)
         if lse is not None:
-            lse = self._vector(lse, torch.float32, n * self._heads, "lse")
+            lse = self._vector(lse, torch.float32, (n, self._heads), "lse")
         if batch.index != self._index:
             raise TypeError("the batch lies on another device than the cache")
         size = 0
