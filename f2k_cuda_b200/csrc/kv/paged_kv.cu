@@ -92,6 +92,12 @@ int take_stride(f2k_kv* h, long long given, int heads, const char* name, long lo
     return F2K_OK;
 }
 
+// A call in place reads and writes a row at the same time: with other strides rows would be written before they are read.
+int check_in_place(f2k_kv* h, const void* in, long long in_stride, const void* out, long long out_stride, int n_tokens, const char* names) {
+    if (in != out || in_stride == out_stride || n_tokens == 1) return F2K_OK;
+    return fail(h, F2K_ERR_INVALID, std::string(names) + " are the same memory with different strides");
+}
+
 struct Workspace {
     size_t join, ml, o, bytes;
 };
@@ -233,6 +239,7 @@ int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const f2k_kv_append_args
     if (const int rc = take_stride(h, a.k_stride, c.n_kv_heads, "k", p.k_stride)) return rc;
     if (const int rc = take_stride(h, a.v_stride, c.n_kv_heads, "v", p.v_stride)) return rc;
     if (const int rc = take_stride(h, a.q_out_stride, c.n_heads, "q_out", p.qo_stride)) return rc;
+    if (const int rc = check_in_place(h, a.q, p.q_stride, a.q_out, p.qo_stride, p.batch.n_tokens, "q and q_out")) return rc;
     p.q = a.q, p.k = a.k, p.v = a.v, p.gamma_q = a.gamma_q, p.gamma_k = a.gamma_k, p.cos_tab = a.cos_table, p.sin_tab = a.sin_table;
     p.k_scale = c.k_scale, p.v_scale = c.v_scale, p.q_out = a.q_out, p.k_pages = c.k_pages, p.v_pages = c.v_pages;
     p.kp_page = c.k_page_stride, p.kp_head = c.k_head_stride, p.kp_tok = c.k_token_stride;
@@ -261,6 +268,7 @@ int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const f2k_kv_attend_args
     if (misaligned(a.lse, 4)) return fail(h, F2K_ERR_INVALID, "lse must be 4-byte aligned");
     if (const int rc = take_stride(h, a.q_stride, c.n_heads, "q", p.q_stride)) return rc;
     if (const int rc = take_stride(h, a.o_stride, c.n_heads, "o", p.o_stride)) return rc;
+    if (const int rc = check_in_place(h, a.q, p.q_stride, a.o, p.o_stride, p.batch.n_tokens, "q and o")) return rc;
     p.q = a.q, p.o = a.o, p.lse = a.lse, p.k_scale = c.k_scale, p.v_scale = c.v_scale;
     p.n_heads = c.n_heads, p.n_kv_heads = c.n_kv_heads, p.group = group_of(h), p.page_shift = h->page_shift, p.n_pages = c.n_pages;
     p.window = c.window, p.scale_log2 = h->scale * 1.4426950408889634f, p.status = h->d_status;

@@ -436,7 +436,7 @@ typedef struct f2k_kv_batch {
 } f2k_kv_batch;
 
 /* What f2k_kv_append takes beside the batch. q, q_out: [n_tokens][n_heads][head_dim], k, v: [n_tokens][n_kv_heads]
- * [head_dim]; q_out may be q. gamma_q, gamma_k: [head_dim] gains of a per-head RMSNorm in front of the rotation, or both
+ * [head_dim]; q_out may be q, with its stride. gamma_q, gamma_k: [head_dim] gains of a per-head RMSNorm in front of the rotation, or both
  * NULL for none. cos_table, sin_table: fp32 [n_positions][rot_dim / 2], row = position; not read with rot_dim 0.
  * Strides between token rows in elements (multiples of 8, a token's heads dense); 0 = dense. */
 typedef struct f2k_kv_append_args {
@@ -448,7 +448,7 @@ typedef struct f2k_kv_append_args {
     float eps;
 } f2k_kv_append_args;
 
-/* What f2k_kv_attend takes beside the batch: q, o [n_tokens][n_heads][head_dim] (o may be q), lse fp32
+/* What f2k_kv_attend takes beside the batch: q, o [n_tokens][n_heads][head_dim] (o may be q, with its stride), lse fp32
  * [n_tokens][n_heads] or NULL, token strides as above, and its workspace. */
 typedef struct f2k_kv_attend_args {
     const void* q;

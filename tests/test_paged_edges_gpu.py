@@ -121,3 +121,20 @@ def test_small_scales_of_the_scores_over_e4m3():
             p.q[0] = 0
             p.attend()
             p.check_attend()
+
+
+@pytest.mark.parametrize("news,lens", [([1, 3, 2], [5000, 70, 900]), ([40, 200, 1], [2000, 200, 5])], ids=["tokens", "prompts"])
+def test_a_layer_in_place_in_wider_rows(news, lens):
+    """Q, K and V are columns of one projection; Q is turned where it stands, and its rows become the attention's."""
+    p = Problem(news, lens, 8, 2, 128, 16, BF, rot=128, gap=520, seed=51)
+    angle = torch.rand(max(lens), 64, generator=p.gen, device="cuda") * 100
+    tables = angle.cos(), angle.sin()
+    apart, o = torch.empty(p.T, 8, 128, device="cuda", dtype=BF), torch.empty(p.T, 8, 128, device="cuda", dtype=BF)
+    assert p.kv.append(p.q, p.k, p.v, (None, None), tables, 1e-6, apart, p.batch)
+    assert p.kv.attend(apart, o, p.batch, p.ws, lse=p.lse)
+    assert p.kv.append(p.q, p.k, p.v, (None, None), tables, 1e-6, p.q, p.batch)
+    assert torch.equal(p.q, apart)
+    assert p.kv.attend(p.q, p.q, p.batch, p.ws, lse=p.lse)
+    assert torch.equal(p.q, o) and p.kv.device_status() == 0
+    assert not p.kv.append(p.q, p.k, p.v, (None, None), tables, 1e-6, p.q.as_strided((p.T, 8, 128), (1024, 128, 1)), p.batch)
+    assert "different strides" in p.kv.last_error()
