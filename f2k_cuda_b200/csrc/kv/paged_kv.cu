@@ -288,7 +288,7 @@ int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const f2k_kv_attend_args
     const int unit = token_unit_keys(c.head_dim * (c.cache_type == F2K_E4M3 ? 1 : 2));
     const long long keys = (long long)batch->table_width << h->page_shift;
     const double tiles = (double)batch->n_tokens * p.group / rows + batch->n_seqs;
-    if (tiles * c.n_kv_heads * (double)(keys / unit + 1 + kWorkCost) >= 4294967295.0)
+    if (tiles * c.n_kv_heads * (double)(keys / unit + 1 + kWorkCost) >= (double)kMostPlaces)
         return fail(h, F2K_ERR_UNSUPPORTED, "the batch could hold 2^32 pieces of work: make two calls of it");
     uint8_t* w = static_cast<uint8_t*>(a.workspace);
     p.ws_join = reinterpret_cast<JoinJob*>(w + ws.join);

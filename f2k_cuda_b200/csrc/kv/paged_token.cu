@@ -122,8 +122,8 @@ paged_token_kernel(const __grid_constant__ AttendParams p) {
         if (w < warp) upto += ctl.scan[w];
         all_places += ctl.scan[w];
     }
-    const unsigned total = all_places >> 32 ? 0u : (unsigned)all_places;
-    if (all_places >> 32 && threadIdx.x == 0) atomicOr(p.status, (int)kStatusBadLength);
+    const unsigned total = all_places > kMostPlaces ? 0u : (unsigned)all_places;
+    if (all_places > kMostPlaces && threadIdx.x == 0) atomicOr(p.status, (int)kStatusBadLength);
     const int n_pieces = pieces(total, p.n_ctas, kLeastPlaces);
     const int cta = blockIdx.x;
     if (cta >= n_pieces || total == 0) {

@@ -16,6 +16,8 @@ constexpr unsigned kWorkCost = 8;
 // A CTA gets at least so many places. One sequence of 1000 keys, 8 heads: 10.6, 9.7, 9.8 us with 12, 8, 6; 47 sequences of up to
 // 18 keys, one head: 10.4, 7.6, 8.8. (A cost of 4: 11.0 and 10.4; 64 sequences of 200 to 8191 keys 125 us, 121 with 8, 123 with 12.)
 constexpr int kLeastPlaces = 8;
+// Places are counted in 32 bits, and a group's walk steps over the end of the line by up to the groups of a CTA.
+constexpr unsigned kMostPlaces = 0xFFFFFF00u;
 
 F2K_HD SeqView seq_of(const PagedBatch& b, int page_shift, int i) {
     return seq_view(b.cu ? b.cu[i] : i, b.cu ? b.cu[i + 1] : i + 1, b.lens[i], b.n_tokens, b.max_new, (long long)b.table_width << page_shift);
