@@ -138,3 +138,69 @@ def test_a_layer_in_place_in_wider_rows(news, lens):
     assert torch.equal(p.q, o) and p.kv.device_status() == 0
     assert not p.kv.append(p.q, p.k, p.v, (None, None), tables, 1e-6, p.q.as_strided((p.T, 8, 128), (1024, 128, 1)), p.batch)
     assert "different strides" in p.kv.last_error()
+
+
+@pytest.mark.parametrize("order", ["longest last", "longest first", "longest in the middle"])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(128, 8, 2), (64, 4, 4)])
+def test_ragged_prompts_in_any_order(order, dim, heads, kv_heads):
+    news = {"longest last": [40, 130, 333, 700, 1500], "longest first": [1500, 700, 333, 130, 40],
+            "longest in the middle": [130, 700, 1500, 333, 40]}[order]
+    p = Problem(news, [n + 77 * b for b, n in enumerate(news)], heads, kv_heads, dim, 64, BF, seed=dim)
+    p.attend()
+    p.check_attend()
+
+
+@pytest.mark.parametrize("cache", [HF, E4], ids=ids)
+def test_more_prompts_than_lanes(cache):
+    """A CTA finds its sequence 32 at a time; some have no new token, one is long."""
+    gen = torch.Generator().manual_seed(8)
+    news = torch.randint(0, 90, (70,), generator=gen).tolist()
+    news[45] = 600
+    p = Problem(news, [n + 13 * b % 200 for b, n in enumerate(news)], 8, 4, 64, 16, HF, cache, seed=9)
+    p.attend()
+    p.check_attend()
+
+
+# one sequence of `new` tokens behind `past` keys, and one beside it
+BATCHES = [(8, 300), (200, 150), (900, 100)]
+
+
+@pytest.mark.parametrize("new,past", BATCHES, ids=["drafts", "a tile", "two tiles"])
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("cache", [BF, E4], ids=ids)
+@pytest.mark.parametrize("value", [float("nan"), float("inf")], ids=["nan", "inf"])
+def test_values_that_are_not_finite_inside_a_sequence(new, past, window, cache, value):
+    """One element of one key and one value, in the middle of a sequence's new tokens. The key is nothing to tokens that do not
+    see it. The value reaches tokens that see it, in its own column, and at most such as lie within 255 tokens of one
+    that does: never another column, key head or sequence."""
+    if cache is E4 and value == float("inf"):
+        pytest.skip("e4m3 has no infinity")
+    p = Problem([new, new], [past + new] * 2, 8, 2, 64, 32, BF, cache, window, seed=new + window)
+    at = past + new // 2
+    pos = torch.arange(past, past + new, device="cuda")
+    sees = (pos >= at) & (pos < at + window if window else True)
+    page, row = int(p.table[0, at // 32]), at % 32
+
+    def out(pages, x):
+        pages[page, 1, row, 5] = x
+        p.attend()
+        assert p.kv.device_status() == 0
+        return p.o.clone(), p.lse.clone()
+
+    (o0, l0), (o1, l1) = out(p.k_pages, 0.0), out(p.k_pages, value)
+    # Rows of a warp move their references together, so the same answers may be rounded in other places: against the formula.
+    p.k_pages[page, 1, row, 5] = 0.0
+    mixed = [torch.cat([torch.where(sees.view(-1, *[1] * (x.dim() - 1)), x[:new], y[:new]), y[new:]]) for x, y in ((o0, o1), (l0, l1))]
+    p.check_attend(*mixed)
+    assert torch.equal(o0[new:], o1[new:]) and torch.equal(o0[:, :4], o1[:, :4])
+    if value != value:
+        assert torch.isnan(o1[:new][sees][:, 4:]).all()
+    out(p.k_pages, 0.0)
+    (o0, l0), (o1, l1) = out(p.v_pages, 0.0), out(p.v_pages, value)
+    assert torch.equal(l0, l1) and torch.equal(o0[new:], o1[new:]) and torch.equal(o0[:, :4], o1[:, :4])
+    others = [c for c in range(64) if c != 5]
+    assert torch.equal(o0[..., others], o1[..., others])
+    assert not torch.isfinite(o1[:new][sees][:, 4:, 5]).any()
+    last = at + window - 1 if window else past + new
+    far = (pos < at - 255) | (pos > last + 255)
+    assert torch.equal(o0[:new][far], o1[:new][far])

@@ -24,16 +24,17 @@ def test_rows_are_parked_behind_the_group_s_queries(dim):
 
 
 def test_a_loader_that_leaves_early_waits_for_every_copy_it_started():
-    """Between the copies of a tile and the next place where the loader can leave, the tile is counted; what is waited for on the
-    way out are the last tiles counted, as many as there are slots. (A tile that is cleared in part reports to a
-    barrier of its own, which is waited for in any case, and counts once it has come.)"""
+    """The places where the loader's loop over the tiles j can be left: in front of tile j's copies with j tiles started; behind
+    them with j + 1, counted before the loop is left. (A 16-bit tile that is cleared in part reports to a barrier of its own, which
+    is waited for in any case.) What is waited for on the way out are the last tiles counted, as many as there are slots."""
     loader = TEXT[TEXT.index("int next_page = look_up(0)"):TEXT.index("constexpr uint32_t idesc_s")]
+    assert "for (; j < n_kv; ++j) {" in loader
     copies = loader.index("tma_load_5d(")
-    counted = re.search(r"if \(bar != smem_u32\(&ctl->clean\)\) issued = j \+ 1;", loader)
-    assert counted and copies < counted.start() < loader.index("break", copies)
     cleared = loader.index("ok = mbar_wait(bar, cleaned & 1")
-    assert cleared < loader.index("++cleaned;\n                    issued = j + 1;")
-    way_out = loader[loader.index("if (!ok) {\n                \n                volatile uint32_t never"):]
+    before, behind = loader[:copies], loader[copies:cleared]
+    assert before.count("break;") == 2 and "++j;" not in before
+    assert re.sub(r"\s+", " ", behind).count("break;") == 1
+    assert "if (!(ok = convert(converted, came_boxes))) { ++j; break; }" in re.sub(r"\s+", " ", behind)
+    way_out = loader[loader.index("volatile uint32_t never"):]
     assert "mbar_wait(smem_u32(&ctl->clean), cleaned & 1, &never" in way_out
-    assert "for (int i = max(0, issued - kSlots); i < issued; ++i)" in way_out
-    assert len(re.findall(r"\bissued = ", loader)) == 2
+    assert "for (int i = max(0, j - kSlots); i < j; ++i)" in way_out
