@@ -44,8 +44,8 @@ struct SeqView {
 };
 F2K_HD SeqView seq_view(int cu0, int cu1, int len, int n_tokens, int max_new, long long capacity) {
     SeqView s;
+    s.first = cu0 < 0 ? 0 : (cu0 > n_tokens ? n_tokens : cu0);
     const bool fits = cu0 >= 0 && cu1 >= cu0 && cu1 <= n_tokens && cu1 - cu0 <= max_new;
-    s.first = fits ? cu0 : 0;
     s.n_new = fits ? cu1 - cu0 : 0;
     s.len = len < 0 ? 0 : (len > capacity ? (int)capacity : len);
     s.bad = !fits || len < s.n_new || len > capacity;
