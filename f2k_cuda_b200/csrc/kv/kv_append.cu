@@ -270,7 +270,7 @@ cudaError_t launch(const AppendParams& p, int sms, cudaStream_t stream) {
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    // While every row can have a team of its own on the GPU at once, it gets one; beyond, eight rows a team, and as many blocks as
+    // While every row can have a team of its own on the GPU at once, it gets one; beyond, four rows a team, and as many blocks as
     // are resident.
     const long long most = (long long)kBlocksPerSm * sms;
     if (rows <= most * kTeams) {

@@ -120,6 +120,8 @@ int group_of(const f2k_kv* h) { return h->cfg.n_heads / h->cfg.n_kv_heads; }
 // e4m3, where the prompt kernel is bound by turning bytes into fp16: 32 rows, 16 sequences of about 27000 keys 348 / 555;
 // 36 and 64 rows alike, of 16000 keys: 8 sequences 224 / 279, 10 sequences 275 / 279, 16 sequences 430 / 282; head_dim 64,
 // 8 sequences 126 / 152, of 1000 keys 24 / 17.
+// More than 64 rows always go to the prompt kernel, few sequences behind many keys too, where its CTAs leave most of the GPU idle: one
+// sequence of 32000 keys, 8 key heads, 64 rows 96 us here, 68 rows 263 there; one key head, 64 rows 48, 80 rows 250.
 bool takes_prompt_kernel(const f2k_kv* h, const f2k_kv_batch* b) {
     const long long rows = (long long)b->max_new * group_of(h);
     if (b->max_new == 1 || rows <= 16) return false;

@@ -13,15 +13,16 @@
 //
 // Roles as in the joint-attention kernel (attn_fwd_sm100.cu): warps 0-3 / 4-7 the softmax groups (one thread per row),
 // warps 8 and 10 the loaders of K and V, warp 9 the tcgen05 issuer, P from tensor memory, lazily moved reference maxima. With
-// head_dim 128 tensor memory has one S buffer, which the groups use in turn; with 64 each has its own (Columns), and is then
-// bound by its own softmax: some 2000 clk a step, of which 1024 are the special-function unit's; with one buffer a group
-// waited another 900 to 1200 for its S. What differs from that kernel:
+// head_dim 128 tensor memory has one S buffer, which the groups use in turn; with 64 each has its own (Columns), and a step of
+// both groups takes 2900 clk, of which the special-function unit has work for 2048 (1024 a group); with one buffer a
+// group waited another 900 to 1200 for its S. P is rounded to 16 bits in front of its product, as there; its sum is taken
+// before. What differs from that kernel:
 //
 //  * A loader brings a key tile in page by page: a lane per page and 128-byte piece of head_dim looks its page up (a
 //    tile ahead) and issues its own TMA box. Rows of V that no query of the CTA may see - the rest of the last page,
 //    pages in front of a window, pages outside the cache - hold anything, and 0 * NaN is NaN in a product, so the loader
 //    waits for such a tile and clears them before it hands the tile over. That is the last tile, or the first ones of a
-//    window. K and V have a ring and a loader each: K of the tile after next may come in as soon as S is done with its slot.
+//    window. (A row that some queries of the CTA see stays for all of them.) K and V have a ring and a loader each: K of the tile after next may come in as soon as S is done with its slot.
 //  * Q is fetched by the softmax groups themselves (the rows of a tile are a gather once group is not a power of two).
 //  * Scores are masked by key number, in tensor memory, only in tiles that some row of the warp does not see whole.
 //
@@ -30,7 +31,9 @@
 // queries are brought into fp16's range by a power of two per row, which goes into the row's exponent factor with the
 // head's scale of K. (8192 tokens 582 us; 6.6 ms in the token kernel, which converts in registers for every 64 rows anew.)
 //
-// Long tiles first: the grid's first CTAs are the last tiles of every sequence, which see the most keys.
+// Long tiles first, inside a sequence: its first CTAs are its last tiles, which see the most keys. The sequences stand in the
+// batch's order, so a batch starts its longest CTAs where its longest prompt stands (8 prompts of 60 to 3000 tokens: 93 us with
+// the longest first, 100 with it last, 109 with it in the middle).
 #include "../attn_params.h"
 #include "../barrier_look.h"
 #include "../ptx.cuh"
@@ -54,6 +57,8 @@ constexpr uint32_t kTmemCols = 512;
 constexpr float kLazyThreshold = 8.0f;                  // log2 units
 constexpr int kPParts = 2;
 // Registers a thread, softmax groups and the other warps, of the 384 * 168 a CTA is launched with; the e4m3 loaders convert.
+// Every variant spills a little (24 to 40 bytes of stack; 72 to 88 bytes loaded with 16-bit caches, 120 to 184 with e4m3).
+// (e4m3 with 208 for the softmax: 8192 tokens 567 instead of 580 us, but with head_dim 64 1024 behind 15001 170 instead of 156.)
 template <bool kE4m3>
 constexpr int kRegsSoftmax = kE4m3 ? 216 : 224;
 template <bool kE4m3>

@@ -16,7 +16,8 @@
 //    exponential was spent on rows that do not exist (96 sequences of about 2700 keys, e4m3, 40 heads over 8: 193 us).
 //
 // Online softmax per warp, raw scores, exponents of 2, fp32; a row's reference only moves when a score exceeds it by 2^8, so
-// most units need no maximum across lanes. P is rounded to 16 bits for the product, the sum is taken before. Rows
+// most units need no maximum across lanes. P is rounded to 16 bits for the product (the tensor cores take no wider operand
+// beside a 16-bit V; a second product for what the rounding leaves would double V's), the sum is taken before. Rows
 // are masked by key number; values of keys that no row of the tile sees are cleared in registers, so what lies in the
 // rest of a page (NaN included) does not matter.
 //

@@ -407,8 +407,8 @@ typedef struct f2k_kv_config {
     /* strides in elements, multiples of 16 bytes; all three 0: dense in the order above */
     long long k_page_stride, k_head_stride, k_token_stride;
     long long v_page_stride, v_head_stride, v_token_stride;
-    /* e4m3 only: [n_kv_heads] fp32 on the device, positive; an element stands for its value times its
-     * head's scale. NULL: 1. */
+    /* e4m3 only: [n_kv_heads] fp32 on the device, positive and not subnormal; an element stands for its value times
+     * its head's scale. NULL: 1. */
     const float* k_scale;
     const float* v_scale;
 } f2k_kv_config;
@@ -472,15 +472,20 @@ int f2k_kv_append(f2k_kv* h, const f2k_kv_batch* batch, const f2k_kv_append_args
 size_t f2k_kv_workspace_bytes(const f2k_kv* h, const f2k_kv_batch* batch);
 
 /* o = softmax(scale q K^T) V over the keys that each token sees; zero for a token that sees none.
- * lse: the logarithm of the sum of exp(scale q K^T), -inf for none. Tokens of a call do not see values
- * of later tokens, but a value that is not finite can make the outputs of up to 255 tokens before it NaN;
- * what lies in pages beyond kv_lens does not matter. */
+ * lse: the logarithm of the sum of exp(scale q K^T), -inf for none. Scores, maxima, sums and accumulators are fp32; the
+ * weights are rounded to the 16-bit type of the product with V (e4m3 caches: fp16) behind their sum, so that o is off by up to
+ * half a step of that type times sum w |v|, beside its own rounding. The same call gives the same bits every time.
+ * What lies in pages beyond kv_lens, or in front of every token's window, does not matter, whatever it is. A key is nothing
+ * to tokens that do not see it. A value that is not finite makes its column NaN, beside the tokens that see it, in tokens
+ * that are attended in one tile with one of those: up to 255 tokens before the value's, and with a window up to 255 behind
+ * the last that sees it; never in another sequence or key head. */
 int f2k_kv_attend(f2k_kv* h, const f2k_kv_batch* batch, const f2k_kv_attend_args* args, void* stream);
 
 /* Reads and clears the status word of this handle's kernels (0 = clean); synchronises the handle's
  * device. F2K_ERR_DEVICE and a message when it is not zero. */
 int f2k_kv_device_status(f2k_kv* h, int* status_out);
-/* As f2k_attn_set_wait_limits; these kernels wait for nothing outside their thread block. */
+/* As f2k_attn_set_wait_limits; these kernels wait for nothing outside their thread block, and a wait looks at its limit
+ * after 256 misses only, each of which suspends the thread: a short limit changes nothing in calls that go well. */
 int f2k_kv_set_wait_limits(f2k_kv* h, long long in_cta_clk);
 
 /* Library identification string (static storage). */
